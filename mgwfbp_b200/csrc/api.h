@@ -88,6 +88,34 @@ int mgw_group_sumsq(const MgwGroup* group, float* partials, int n_ctas, void* st
 // out[n, j, i, p*6 + q*3 + c] = x[n, 2j + p - 4, 2i + q - 4, c].
 int mgw_s2d_stem_input(const float* x, float* out, int N, int H, int W, void* stream);
 
+// ---- embedding lookup and its gradient (embedding.cu) -------------------------------------------------
+// dtype: MGW_F32 / MGW_F16 / MGW_BF16 (dtypes.cuh); tokens: int32 (wide = 0) or int64 (wide = 1).  A token outside
+// [0, vocab) is recorded in `status` (mgw_token_status) and gives a row of NaN, or no contribution to the gradient.
+int mgw_token_status(int** words_out);                               // 8 pinned words, one block per process
+int mgw_embedding_fwd(const void* tokens, int wide, long long n, const void* weight, long long ld, long long vocab, int dim, int dtype,
+                      float scale, void* out, int* status, void* stream);
+size_t mgw_embedding_grad_bytes(long long n, long long vocab, int dim, int dtype);      // scratch memory of the call below
+// dw [vocab, dim] is written whole; rows of the token `padding` (-1: none) stay zero.
+int mgw_embedding_grad(const void* dy, long long dy_ld, const void* tokens, int wide, long long n, long long vocab, int dim, int dtype,
+                       float scale, long long padding, void* dw, void* work, size_t work_bytes, int* status, void* stream);
+
+// ---- log probabilities, entropy, likeliest tokens, cross entropy (logprob.cu) -------------------------
+// stats: [rows][2] largest logit and logarithm of the sum of exp(z - it), for the backward pass (may be null).
+int mgw_logprob_fwd(const void* z, long long ld, long long rows, int vocab, int dtype, const void* tokens, int wide, long long ignore,
+                    float* logprob, float* entropy, float* stats, int top, float* top_logprob, long long* top_tokens, int* status,
+                    void* stream);
+int mgw_logprob_bwd(const void* z, long long ld, long long rows, int vocab, int dtype, const void* tokens, int wide, long long ignore,
+                    const float* stats, const float* entropy, const float* g_logprob, const float* g_entropy, const float* g_loss,
+                    const float* count, void* dz, long long dz_ld, void* stream);
+int mgw_mean_loss(const float* logprob, const void* tokens, int wide, long long ignore, long long rows, int mean, float* loss, float* count,
+                  void* stream);
+
+// ---- global gradient norm and clipping (grad_clip.cu) -------------------------------------------------
+// norm: 0 two-norm, 1 sum of magnitudes, 2 largest magnitude; clip = 0 only measures.  work: mgw_grad_clip_bytes(n).
+size_t mgw_grad_clip_bytes(int n);
+int mgw_grad_clip(const unsigned long long* ptrs, const long long* numels, const unsigned char* dtypes, int n, int norm, double scale,
+                  double max_norm, int clip, void* work, size_t work_bytes, float* norm_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

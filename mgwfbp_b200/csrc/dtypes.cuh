@@ -1,0 +1,71 @@
+// Element types of the language-model operators and vector accesses to them: values are held in fp32 inside the kernels
+// and rounded (to nearest even) once when they are stored.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "common.cuh"
+
+// codes of the C interface
+#define MGW_F32 0
+#define MGW_F16 1
+#define MGW_BF16 2
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ float mgw_to_float(float x) { return x; }
+__device__ __forceinline__ float mgw_to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float mgw_to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T> __device__ __forceinline__ T mgw_from_float(float x);
+template <> __device__ __forceinline__ float mgw_from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half mgw_from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 mgw_from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// N values of type T that move as one access of N * sizeof(T) bytes (2, 4, 8 or 16)
+template <int BYTES> struct MgwRaw;
+template <> struct MgwRaw<16> { typedef uint4 type; };
+template <> struct MgwRaw<8> { typedef uint2 type; };
+template <> struct MgwRaw<4> { typedef uint32_t type; };
+template <> struct MgwRaw<2> { typedef uint16_t type; };
+
+template <typename T, int N>
+union MgwVec {
+    typename MgwRaw<N * sizeof(T)>::type raw;
+    T v[N];
+    __device__ __forceinline__ MgwVec() {}
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void mgw_unpack(const typename MgwRaw<N * sizeof(T)>::type& raw, float (&f)[N]) {
+    MgwVec<T, N> u;
+    u.raw = raw;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = mgw_to_float(u.v[i]);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ typename MgwRaw<N * sizeof(T)>::type mgw_pack(const float (&f)[N]) {
+    MgwVec<T, N> u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) u.v[i] = mgw_from_float<T>(f[i]);
+    return u.raw;
+}
+
+__device__ __forceinline__ float mgw_nan() { return __int_as_float(0x7fc00000); }
+
+// The token with index i of an int32 (wide = 0) or int64 (wide = 1) list.
+__device__ __forceinline__ long long mgw_token(const void* tokens, int wide, long long i) {
+    return wide ? static_cast<const long long*>(tokens)[i] : (long long)static_cast<const int*>(tokens)[i];
+}
+
+// Record a token outside the vocabulary: {MGW_STATUS_BOUNDS, operator, position, token, cta}, the first one wins.
+#define MGW_OP_EMBEDDING 1
+#define MGW_OP_EMBEDDING_GRAD 2
+#define MGW_OP_LOGPROB 3
+__device__ __forceinline__ void mgw_report_token(int* status, int op, long long position, long long token) {
+    const long long lo = -2147483647LL - 1, hi = 2147483647LL;
+    mgw_report(status, MGW_STATUS_BOUNDS, op, (int)(position < hi ? position : hi),
+               (int)(token < lo ? lo : token > hi ? hi : token));
+}
+
+#endif  // __CUDACC__

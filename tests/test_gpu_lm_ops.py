@@ -1,0 +1,557 @@
+"""Embedding, token log probabilities, cross entropy and gradient clipping on the GPU against 64-bit evaluations, with the
+bounds that ``lm_oracle`` derives."""
+import math
+
+import pytest
+import torch
+
+from lm_oracle import Rows, U, assert_within, embedding_grad as oracle_grad, half_step, tiny
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+ids = lambda v: str(v).replace('torch.', '') if isinstance(v, torch.dtype) else None      # noqa: E731
+
+
+def _tokens(kind, n, vocab, gen):
+    if kind == 'same':
+        return torch.full((n,), vocab // 2, device='cuda')
+    if kind == 'zipf':
+        u = torch.rand(n, device='cuda', generator=gen)
+        return (torch.exp(u * math.log(vocab + 1)) - 1).long().clamp_(0, vocab - 1)
+    if kind == 'last':
+        return torch.full((n,), vocab - 1, device='cuda')
+    return torch.randint(0, vocab, (n,), device='cuda', generator=gen)
+
+
+# ---------------------------------------------------------------------------------------------------------- embedding
+@pytest.mark.parametrize('dtype', TYPES, ids=ids)
+@pytest.mark.parametrize('n,vocab,dim,kind', [
+    (1, 1, 1, 'any'), (1, 10, 4, 'any'), (2, 3, 7, 'same'), (7, 5, 33, 'any'), (31, 100, 128, 'last'), (33, 2, 130, 'any'),
+    (700, 1000, 1500, 'zipf'), (2047, 257, 1023, 'zipf'), (2049, 70000, 8, 'any'), (4099, 33, 258, 'zipf'), (5000, 300, 640, 'same'),
+    (20011, 5003, 129, 'zipf'), (40000, 131072, 24, 'zipf')])
+def test_embedding_forward_and_gradient(n, vocab, dim, kind, dtype):
+    from mgwfbp_b200.ops.embedding import check_status, embedding
+    gen = torch.Generator(device='cuda').manual_seed(n)
+    t = _tokens(kind, n, vocab, gen)
+    t = t.int() if n % 2 else t
+    w = torch.randn(vocab, dim, device='cuda', generator=gen).to(dtype).requires_grad_()
+    for scale, padding in ((1.0, None), (math.sqrt(dim) + 0.1, int(t[0]))):
+        out = embedding(t, w, scale, padding)
+        want = w.detach()[t.long()].double() * scale
+        if scale == 1.0:
+            assert torch.equal(out, w.detach()[t.long()])
+        # the factor and the product round in fp32, the result to the type
+        assert_within(out, want, want.abs() * (half_step(dtype) + 2.001 * U) + tiny(dtype), 'out')
+        dy = torch.randn(n, dim, device='cuda', generator=gen).to(dtype)
+        (dw,) = torch.autograd.grad(out, w, dy)
+        want, bound = oracle_grad(dy, t, vocab, scale, padding)
+        assert_within(dw, want, bound, 'dw')
+        (again,) = torch.autograd.grad(embedding(t, w, scale, padding), w, dy)
+        assert torch.equal(dw, again)                                            # the same on every run
+    check_status()
+
+
+def test_embedding_strides_shapes_and_broadcast_gradient():
+    from mgwfbp_b200.ops.embedding import embedding, embedding_grad
+    wide = torch.randn(50, 40, device='cuda')
+    t = torch.randint(0, 50, (6, 8), device='cuda').t()                          # not contiguous
+    for cols in (slice(0, 32), slice(1, 33), slice(3, 20)):                      # rows further apart, odd starts
+        w = wide[:, cols].detach().requires_grad_()
+        out = embedding(t, w)
+        assert out.shape == (8, 6, w.shape[1]) and torch.equal(out, w.detach()[t])
+        (dw,) = torch.autograd.grad(out.sum(), w)                                # a gradient of stride zero
+        want = torch.bincount(t.reshape(-1), minlength=50).float().unsqueeze(1).expand(50, w.shape[1])
+        assert torch.equal(dw, want)
+    dy = torch.randn(8, 6, 96, device='cuda')[..., 5:69]
+    want, bound = oracle_grad(dy, t, 50, 1.0)
+    assert_within(embedding_grad(dy, t, 50), want, bound, 'strided dy')
+    w = wide.t().detach().requires_grad_()                                       # columns of another matrix
+    t2 = torch.tensor([0, 39, 39], device='cuda')
+    out = embedding(t2, w, 3.0)
+    assert_within(out, w.detach()[t2].double() * 3, out.double().abs() * 2 * U, 'transposed table')
+
+
+@pytest.mark.parametrize('n', [5, 3000, 9000])
+def test_embedding_nan_stays_in_its_row(n):
+    from mgwfbp_b200.ops.embedding import embedding_grad
+    t = torch.arange(n, device='cuda') % 100
+    dy = torch.ones(n, 20, device='cuda')
+    dy[4] = math.nan                                                             # token 4
+    dw = embedding_grad(dy, t, 101, padding_idx=4)
+    assert torch.isfinite(dw).all() and not dw[4].any() and not dw[100].any()
+    dw = embedding_grad(dy, t, 101)
+    assert dw[4].isnan().all() and torch.isfinite(dw[:4]).all() and torch.isfinite(dw[5:]).all()
+
+
+@pytest.mark.parametrize('n', [6, 5000])
+def test_token_outside_the_vocabulary_is_reported(n):
+    from mgwfbp_b200.ops import embedding as emb, logprob as lp
+    w = torch.randn(10, 12, device='cuda')
+    t = torch.arange(n, device='cuda') % 10
+    emb.check_status()
+    for bad in (10, -1, 1 << 40):
+        t[3] = bad
+        out = emb.embedding(t, w)
+        assert out[3].isnan().all() and torch.equal(out[:3], w[t[:3]]) and torch.equal(out[4:], w[t[4:]])
+        with pytest.raises(emb.TokenIndexError, match='position 3'):
+            emb.check_status()
+        dw = emb.embedding_grad(torch.ones(n, 12, device='cuda'), t, 10)
+        with pytest.raises(emb.TokenIndexError, match='gradient'):
+            emb.check_status()
+        ok = torch.cat([t[:3], t[4:]])
+        assert torch.equal(dw, torch.bincount(ok, minlength=10).float().unsqueeze(1).expand(10, 12))
+        z = torch.randn(n, 10, device='cuda', requires_grad=True)
+        r = lp.token_log_probs(z, t)
+        assert r.logprob[3].isnan() and torch.isfinite(r.logprob[:3]).all() and torch.isfinite(r.entropy).all()
+        with pytest.raises(lp.TokenIndexError, match='log prob'):
+            lp.check_status()
+        (dz,) = torch.autograd.grad(r.logprob.sum(), z)
+        assert dz[3].isnan().all() and torch.isfinite(dz[:3]).all() and torch.isfinite(dz[4:]).all()
+        assert lp.cross_entropy(z, t).isnan()
+        with pytest.raises(lp.TokenIndexError):
+            lp.check_status()
+    emb.check_status()
+
+
+def test_embedding_offsets_beyond_32_bits():
+    from mgwfbp_b200.ops.embedding import embedding, embedding_grad
+    w = torch.zeros(70000, 65536, dtype=torch.bfloat16, device='cuda')           # 4.6e9 elements
+    w[69999, :] = 3.0
+    w[40000, 5] = 2.0
+    out = embedding(torch.tensor([69999, 40000, 0], device='cuda'), w)
+    assert (out[0] == 3).all() and out[1, 5] == 2 and out[1].sum() == 2 and not out[2].any()
+    del w
+    dw = embedding_grad(out, torch.tensor([69999, 40000, 69999], device='cuda'), 70000)
+    assert (dw[69999] == 3).all() and dw[40000, 5] == 2 and dw[40000].sum() == 2
+    dw[69999] = 0
+    dw[40000] = 0
+    assert not dw.any()
+
+
+# ----------------------------------------------------------------------------------------------------- log probabilities
+def _case(rows, vocab, pad, dtype, seed, special=True):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    wide = (torch.randn(rows, vocab + pad, device='cuda', generator=gen) * 4).to(dtype)
+    z = wide[:, :vocab]
+    t = torch.randint(0, vocab, (rows,), device='cuda', generator=gen)
+    if special:
+        low = torch.finfo(dtype).min
+        for r in range(rows):
+            k = r % 12
+            keep = int(t[r])
+            if k == 1:                                     # only a few tokens allowed
+                z[r, torch.rand(vocab, device='cuda', generator=gen) < 0.9] = -math.inf
+                z[r, keep] = 1.0
+            elif k == 2:                                   # masked with the type's lowest value
+                z[r, torch.rand(vocab, device='cuda', generator=gen) < 0.5] = low
+                z[r, keep] = 0.5
+            elif k == 3:
+                z[r] = 1.5                                 # all equal
+            elif k == 4:
+                t[r] = -100
+                z[r] = math.nan                            # padding: never read
+            elif k == 5:
+                z[r] = -math.inf                           # nothing left
+            elif k == 6:
+                z[r, keep] = math.nan
+            elif k == 7:
+                z[r, vocab // 2] = math.inf
+            elif k == 8:
+                z[r] = low                                 # all at the lowest value: all equal
+            elif k == 9:
+                z[r] = -math.inf
+                z[r, keep] = -3.0                          # one token left
+            elif k == 10:
+                z[r] += 500.0                              # far from zero
+            elif k == 11:
+                z[r] = z[r].abs() * 0.0                    # zeros of both signs
+                z[r, ::2] *= -1.0
+    return z, t
+
+
+SHAPES = [(1, 1, 0), (3, 2, 0), (13, 31, 1), (13, 127, 0), (12, 128, 0), (26, 1000, 0), (12, 1024, 8), (24, 10000, 0), (25, 10001, 0),
+          (13, 50261, 43), (12, 32768, 0), (12, 131072, 0), (1, 100003, 0)]
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=ids)
+@pytest.mark.parametrize('rows,vocab,pad', SHAPES)
+def test_log_probs_and_gradient(rows, vocab, pad, dtype):
+    from mgwfbp_b200.ops.logprob import check_status, token_log_probs
+    z, t = _case(rows, vocab, pad, dtype, rows * 7 + vocab)
+    z = z.detach().requires_grad_()
+    want = Rows(z, t)
+    for top in sorted({0, 1, min(5, vocab), min(20, vocab), min(32, vocab)}):
+        r = token_log_probs(z, t if top % 2 else t.int(), top=top)
+        assert_within(r.logprob, *want.logprob(), 'logprob')
+        assert_within(r.entropy, *want.entropy(), 'entropy')
+        v, bound, order = want.top(top)
+        assert torch.equal(r.top_tokens, order), top
+        assert_within(r.top_logprob, v, bound, 'top')
+    g1, g2 = torch.randn(rows, device='cuda'), torch.randn(rows, device='cuda')
+    zero = torch.zeros(rows, device='cuda')
+    for outs, gs, ws in (([r.logprob, r.entropy], [g1, g2], (g1, g2)), ([r.logprob], [g1], (g1, zero)), ([r.entropy], [g2], (zero, g2))):
+        (dz,) = torch.autograd.grad(outs, [z], gs, retain_graph=True)
+        assert dz.dtype == dtype
+        w, bound = want.grad(*ws, dtype)
+        assert_within(dz, w, bound, 'dz')
+    check_status()
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=ids)
+@pytest.mark.parametrize('rows,vocab,pad', SHAPES)
+@pytest.mark.parametrize('reduction,upstream', [('mean', 1.0), ('mean', 128.0), ('sum', -0.37)])
+def test_cross_entropy_and_gradient(rows, vocab, pad, dtype, reduction, upstream):
+    from mgwfbp_b200.ops.logprob import check_status, cross_entropy
+    z, t = _case(rows, vocab, pad, dtype, rows * 11 + vocab, special=False)
+    if rows > 2:
+        t[1::3] = -100
+    z = z.detach().requires_grad_()
+    want = Rows(z, t)
+    lp, bound = want.logprob()
+    n = int((t != -100).sum()) if reduction == 'mean' else 1
+    for expected in (1.0, upstream):
+        loss = cross_entropy(z, t, reduction=reduction, expected_grad=expected)
+        assert loss.dtype == torch.float32 and loss.dim() == 0
+        # the rows' errors, and one rounding of the 64-bit sum
+        assert_within(loss, -lp.sum() / n, bound[t != -100].sum() / n + U * (lp.sum().abs() / n) * 1.01, 'loss')
+        up = torch.tensor(upstream, device='cuda')
+        (dz,) = torch.autograd.grad(loss, z, up, retain_graph=True)
+        g = torch.full((rows,), -upstream / n, dtype=torch.float64, device='cuda')
+        w, b = want.grad(g, torch.zeros_like(g), dtype)
+        assert_within(dz, w, b, 'dz')
+        (again,) = torch.autograd.grad(loss, z, up)                              # a graph that was kept
+        assert torch.equal(dz, again)
+    check_status()
+
+
+def test_cross_entropy_special_rows():
+    from mgwfbp_b200.ops.logprob import FusedCrossEntropyLoss, cross_entropy
+    z, t = _case(12, 500, 0, torch.float32, 5)
+    want = Rows(z, t)
+    lp, bound = want.logprob()
+    assert_within(cross_entropy(z, t, reduction='none'), -lp, bound, 'none')
+    fine = want.fine & ~want.pad
+    zz = z.detach().clone().requires_grad_()
+    t2 = torch.where(fine | want.pad, t, torch.full_like(t, -100))              # the rows without a distribution become padding
+    loss = FusedCrossEntropyLoss()(zz, t2)
+    loss.backward()
+    ref = z.detach()[fine].double().requires_grad_()
+    torch.nn.functional.cross_entropy(ref, t[fine]).backward()
+    assert not zz.grad[~fine].any()
+    torch.testing.assert_close(zz.grad[fine].double(), ref.grad, rtol=1e-4, atol=1e-6)
+    every = torch.full_like(t, -100)
+    zz.grad = None
+    loss = cross_entropy(zz, every)
+    loss.backward()
+    assert loss.isnan() and not zz.grad.any()
+    assert cross_entropy(zz, every, reduction='sum') == 0
+
+
+def test_gradients_against_differences():
+    """Directional derivative by central differences of the 64-bit functions."""
+    from mgwfbp_b200.ops.logprob import token_log_probs
+    z, t = _case(6, 301, 0, torch.float32, 3, special=False)
+    z = z.detach().requires_grad_()
+    r = token_log_probs(z, t)
+    (dz,) = torch.autograd.grad((r.logprob + 0.5 * r.entropy).sum(), z)
+    v = torch.randn_like(z).double()
+    f = lambda s: sum(float(x.sum()) * k for x, k in ((Rows(z.detach().double() + s * v, t).logprob()[0], 1.0),      # noqa: E731
+                                                      (Rows(z.detach().double() + s * v, t).entropy()[0], 0.5)))
+    got, want = float((dz.double() * v).sum()), (f(1e-5) - f(-1e-5)) / 2e-5
+    assert abs(got - want) <= 1e-4 * max(1.0, float((dz.double() * v).abs().sum()))
+
+
+def test_log_probs_shapes_and_strides():
+    from mgwfbp_b200.ops.logprob import token_log_probs
+    z = torch.randn(4, 5, 64, device='cuda')
+    t = torch.randint(0, 64, (4, 5), device='cuda')
+    r = token_log_probs(z, t, top=3)
+    assert r.logprob.shape == r.entropy.shape == (4, 5) and r.top_tokens.shape == r.top_logprob.shape == (4, 5, 3)
+    want = Rows(z, t)
+    assert_within(r.logprob.reshape(-1), *want.logprob(), 'batched')
+    zt = z.transpose(0, 1).detach().requires_grad_()                             # rows in another order
+    q = token_log_probs(zt, t.t(), top=3)
+    assert torch.equal(q.logprob, r.logprob.t()) and torch.equal(q.top_tokens, r.top_tokens.transpose(0, 1))
+    (dz,) = torch.autograd.grad(q.logprob.sum(), zt)
+    assert dz.shape == zt.shape
+    cols = torch.randn(64, 7, device='cuda').t()                                 # columns of another matrix
+    c = token_log_probs(cols, t.reshape(-1)[:7])
+    assert torch.equal(c.logprob, token_log_probs(cols.contiguous(), t.reshape(-1)[:7]).logprob)
+    e = token_log_probs(torch.randn(1, 64, device='cuda').expand(6, 64), torch.zeros(6, dtype=torch.int64, device='cuda'))
+    assert (e.logprob == e.logprob[0]).all()
+    none = token_log_probs(z[:0], t[:0], top=2)
+    assert none.logprob.shape == (0, 5) and none.top_tokens.shape == (0, 5, 2)
+
+
+def test_log_probs_offsets_beyond_32_bits():
+    from mgwfbp_b200.ops.logprob import token_log_probs
+    ld = 1_200_000_000
+    store = torch.empty(2 * ld + 1000, dtype=torch.bfloat16, device='cuda')
+    z = store.as_strided((3, 1000), (ld, 1))
+    z.copy_(torch.randn(3, 1000, device='cuda'))
+    t = torch.tensor([1, 2, 3], device='cuda')
+    want = Rows(z, t)
+    r = token_log_probs(z.detach().requires_grad_(), t, top=4)
+    assert_within(r.logprob, *want.logprob(), 'logprob')
+    assert torch.equal(r.top_tokens, want.top(4)[2])
+    zz = z.detach().requires_grad_()
+    (dz,) = torch.autograd.grad(token_log_probs(zz, t).logprob.sum(), zz)
+    assert dz.is_contiguous()                                                    # not as far apart as the logits
+    one = torch.ones(3, device='cuda')
+    assert_within(dz, *want.grad(one, one * 0, torch.bfloat16), 'dz')
+
+
+# ------------------------------------------------------------------------------------------------------------- clipping
+def _grads(sizes, dtypes, gen, sd=1.0, offset=0):
+    """Tensors one behind the other in one buffer per type, so that their addresses have every alignment."""
+    out = []
+    for dt in dtypes:
+        mine = [n for i, n in enumerate(sizes) if dtypes[i % len(dtypes)] == dt]
+        flat = (torch.randn(sum(mine) + offset, device='cuda', generator=gen) * sd).to(dt)
+        at = offset
+        for n in mine:
+            out.append(flat[at:at + n])
+            at += n
+    return out
+
+
+def _exact_clip(grads, max_norm, norm_type, scale):
+    each = torch.cat([g.double().reshape(-1) for g in grads]) * scale
+    norm = torch.linalg.vector_norm(each, norm_type)
+    c = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
+    return norm, [g.double() * scale * c for g in grads]
+
+
+@pytest.mark.parametrize('norm_type', [2.0, 1.0, math.inf])
+@pytest.mark.parametrize('sizes,dtypes,offset', [
+    ([1], [torch.float32], 0), ([1, 2, 3, 5, 7], [torch.bfloat16], 1), ([5], [torch.float16], 3), ([0, 8192, 0, 8193, 8191], [torch.float32], 1),
+    ([100003, 17, 16384 * 3 + 5, 4], TYPES, 5), ([7] * 130, [torch.bfloat16, torch.float32], 0), ([33] * 1100, [torch.float16], 0),
+    ([3_000_001, 5_000_003], [torch.bfloat16], 0), ([20_000_000], [torch.float32], 2)])
+def test_clip_and_norm(sizes, dtypes, offset, norm_type):
+    from mgwfbp_b200.ops.clip import clip_grad_norm_, grad_norm
+    gen = torch.Generator(device='cuda').manual_seed(len(sizes))
+    for scale, limit in ((1.0, 0.3), (2.0, 0.01), (0.125, 1e30)):
+        grads = _grads(sizes, dtypes, gen, offset=offset)
+        want_norm, want = _exact_clip(grads, limit, norm_type, scale)
+        params = [torch.nn.Parameter(torch.empty_like(g)) for g in grads]
+        for p, g in zip(params, grads):
+            p.grad = g
+        before = grad_norm(grads, norm_type, scale)
+        norm = clip_grad_norm_(params, limit, norm_type, grad_scale=scale)
+        # 64-bit sums: what is left is the rounding of the norm to fp32
+        assert_within(norm, want_norm, want_norm * U * 1.01, 'norm')
+        assert torch.equal(norm, before)
+        for g, w in zip(grads, want):                          # the factor and the product round in fp32, the result to the type
+            assert_within(g, w, w.abs() * (half_step(g.dtype) + 2.1 * U) + tiny(g.dtype), 'grad')
+
+
+def test_clip_leaves_small_gradients_alone():
+    from mgwfbp_b200.ops.clip import clip_grad_norm_
+    p = torch.nn.Parameter(torch.zeros(1000, device='cuda'))
+    p.grad = torch.randn(1000, device='cuda')
+    keep = p.grad.clone()
+    clip_grad_norm_([p], 1e6)
+    assert torch.equal(p.grad, keep)
+
+
+def test_clip_values_whose_squares_leave_fp32():
+    from mgwfbp_b200.ops.clip import clip_grad_norm_
+    for v in (1e-30, 1e30, 3e38, 1e-42):
+        p = torch.nn.Parameter(torch.zeros(64, device='cuda'))
+        p.grad = torch.full((64,), v, device='cuda')
+        x = float(p.grad[0])
+        norm = clip_grad_norm_(p, 1.0)
+        want = 8.0 * x
+        if want <= torch.finfo(torch.float32).max:
+            assert abs(float(norm) - want) <= want * U * 1.01 + tiny(torch.float32)
+        else:
+            assert math.isinf(float(norm))
+        w = torch.full((64,), x * min(1.0, 1.0 / (want + 1e-6)), dtype=torch.float64)
+        assert_within(p.grad, w, w * 3.1 * U + 2 * tiny(torch.float32), 'grad')
+
+
+@pytest.mark.parametrize('value', [math.nan, math.inf])
+@pytest.mark.parametrize('norm_type', [2.0, 1.0, math.inf])
+def test_clip_nonfinite_is_the_librarys(value, norm_type):
+    from mgwfbp_b200.ops.clip import clip_grad_norm_
+    mine = [torch.nn.Parameter(torch.zeros(n, device='cuda')) for n in (5, 70000)]
+    theirs = [torch.nn.Parameter(torch.zeros(n, device='cuda')) for n in (5, 70000)]
+    for p, q in zip(mine, theirs):
+        p.grad = torch.randn_like(p)
+        q.grad = p.grad.clone()
+    for ps in (mine, theirs):
+        ps[1].grad[69999] = value
+    keep = mine[0].grad.clone()
+    with pytest.raises(RuntimeError, match='non-finite'):
+        clip_grad_norm_(mine, 1.0, norm_type, error_if_nonfinite=True)
+    assert torch.equal(mine[0].grad, keep)
+    a, b = clip_grad_norm_(mine, 1.0, norm_type), torch.nn.utils.clip_grad_norm_(theirs, 1.0, norm_type)
+    assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.isinf(), b.isinf())
+    for p, q in zip(mine, theirs):
+        torch.testing.assert_close(p.grad, q.grad, equal_nan=True)
+
+
+def test_clip_layouts_repeats_and_overlaps():
+    from mgwfbp_b200.ops.clip import clip_grad_norm_
+    p = torch.nn.Parameter(torch.zeros(4, 3, 5, 5, device='cuda').contiguous(memory_format=torch.channels_last))
+    p.grad = torch.randn(4, 3, 5, 5, device='cuda').contiguous(memory_format=torch.channels_last)
+    q = torch.nn.Parameter(torch.zeros(8, 6, device='cuda').t())
+    q.grad = torch.randn(8, 6, device='cuda').t()
+    want_norm, want = _exact_clip([p.grad, q.grad], 0.5, 2.0, 1.0)
+    norm = clip_grad_norm_([p, q, p, q], 0.5)                                    # each counts and is scaled once
+    assert_within(norm, want_norm, want_norm * U * 1.01, 'norm')
+    for g, w in zip((p.grad, q.grad), want):
+        assert_within(g, w, w.abs() * 3.1 * U, 'grad')
+    flat = torch.randn(100, device='cuda')
+    a, b = torch.nn.Parameter(torch.zeros(60, device='cuda')), torch.nn.Parameter(torch.zeros(60, device='cuda'))
+    a.grad, b.grad = flat[:60], flat[40:]
+    keep = flat.clone()
+    with pytest.raises(ValueError, match='share memory'):
+        clip_grad_norm_([a, b], 0.1)
+    assert torch.equal(flat, keep)
+    a.grad = torch.randn(1, device='cuda').expand(60)
+    with pytest.raises(ValueError, match='stretch of memory'):
+        clip_grad_norm_([a], 0.1)
+    a.grad, b.grad = flat[:60].clone(), None
+    c = torch.nn.Parameter(torch.zeros(3))
+    c.grad = torch.zeros(3)
+    with pytest.raises(ValueError, match='one device'):
+        clip_grad_norm_([a, c], 0.1)
+
+
+def test_clip_offsets_beyond_32_bits():
+    from mgwfbp_b200.ops.clip import clip_grad_norm_
+    n = (1 << 32) + 12345
+    p = torch.nn.Parameter(torch.empty(0, dtype=torch.bfloat16, device='cuda'))
+    g = torch.zeros(n, dtype=torch.bfloat16, device='cuda')
+    g[-1], g[(1 << 32) - 1], g[0] = 3.0, 4.0, 12.0
+    p.data = g                                                                   # a gradient needs its parameter's shape
+    p.grad = g
+    norm = clip_grad_norm_(p, 6.5)
+    assert float(norm) == 13.0
+    assert float(g[-1]) == 1.5 and float(g[(1 << 32) - 1]) == 2.0 and float(g[0]) == 6.0
+
+
+# -------------------------------------------------------------------------------------------- streams, graphs, together
+def _together(net, tokens, targets):
+    """One training step's operators as a language model calls them."""
+    from mgwfbp_b200.ops.clip import clip_grad_norm_
+    from mgwfbp_b200.ops.embedding import embedding
+    from mgwfbp_b200.ops.logprob import cross_entropy, token_log_probs
+    table, out = net
+    x = embedding(tokens, table, scale=2.0, padding_idx=0)
+    z = x.reshape(-1, x.shape[-1]) @ out
+    loss = cross_entropy(z, targets.reshape(-1), ignore_index=0)
+    dt, do = torch.autograd.grad(loss, [table, out])
+    table.grad, out.grad = dt, do
+    norm = clip_grad_norm_([table, out], 0.05)
+    r = token_log_probs(z.detach(), targets.reshape(-1), top=3, ignore_index=0)
+    return [loss.detach(), norm, dt, do, r.logprob, r.entropy, r.top_logprob, r.top_tokens]
+
+
+def _together_inputs(seed, n=300):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    tokens = torch.randint(0, 501, (n,), device='cuda', generator=gen)
+    tokens[::7] = 0
+    return tokens, torch.roll(tokens, -1)
+
+
+def _together_net():
+    gen = torch.Generator(device='cuda').manual_seed(1)
+    table = (torch.randn(501, 64, device='cuda', generator=gen) * 0.1).requires_grad_()
+    return table, (torch.randn(64, 501, device='cuda', generator=gen) * 0.1).requires_grad_()
+
+
+def test_operators_together_match_64_bits():
+    net, (tokens, targets) = _together_net(), _together_inputs(2)
+    prev = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    try:
+        loss, norm, dt, do, logprob, entropy, tlp, tt = _together(net, tokens, targets)
+    finally:
+        torch.backends.cuda.matmul.allow_tf32 = prev
+    table, out = (p.detach().double().requires_grad_() for p in net)
+    x = torch.nn.functional.embedding(tokens, table, padding_idx=0) * 2.0
+    z = x @ out
+    want = torch.nn.functional.cross_entropy(z, targets, ignore_index=0)
+    want.backward()
+    total = torch.nn.utils.clip_grad_norm_([table, out], 0.05)
+    torch.testing.assert_close(loss.double(), want.detach(), rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(norm.double(), total, rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(dt.double(), table.grad, rtol=1e-4, atol=1e-6)
+    torch.testing.assert_close(do.double(), out.grad, rtol=1e-4, atol=1e-6)
+    keep = targets != 0
+    lp = torch.log_softmax(z.detach(), 1)
+    torch.testing.assert_close(logprob[keep].double(), lp[keep].gather(1, targets[keep, None]).squeeze(1), rtol=1e-5, atol=1e-5)
+    assert not logprob[~keep].any() and (tt[~keep] == -1).all()
+
+
+def test_operators_on_another_stream_and_in_two_graphs():
+    """Two captured graphs replayed in turn and on streams of their own give what eager calls give, bit for bit."""
+    net = _together_net()
+    sets = [_together_inputs(s) for s in (5, 6)]
+    want = [[v.clone() for v in _together(net, *s)] for s in sets]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = _together(net, *sets[1])
+    side.synchronize()
+    for a, b in zip(got, want[1]):
+        assert torch.equal(a, b)
+    graphs, outs, statics = [], [], []
+    for s in sets:
+        static = [v.clone() for v in s]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = _together(net, *static)
+        graphs.append(g)
+        outs.append(o)
+        statics.append(static)
+    for turn in range(3):                                      # the graphs' inputs change places
+        for k in (0, 1):
+            for st, v in zip(statics[k], sets[(k + turn) % 2]):
+                st.copy_(v)
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        for k in (0, 1):                                       # both at once
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            for a, b in zip(outs[k], want[(k + turn) % 2]):
+                assert torch.equal(a, b)
+    from mgwfbp_b200.ops.embedding import check_status
+    check_status()
+
+
+def test_native_launches_are_counted():
+    from mgwfbp_b200.ops import counters
+    before = counters.snapshot()
+    _together(_together_net(), *_together_inputs(3))
+    seen = counters.diff(before)
+    for name in ('embedding_fwd', 'embedding_grad', 'logprob_fwd', 'grad_norm', 'grad_scale'):
+        assert seen.get(name, 0) >= 1, (name, seen)
+
+
+def test_refusals_on_the_gpu():
+    from mgwfbp_b200.ops.clip import grad_norm
+    from mgwfbp_b200.ops.embedding import embedding, embedding_grad
+    from mgwfbp_b200.ops.logprob import token_log_probs
+    w, t = torch.randn(5, 4, device='cuda', dtype=torch.float64), torch.tensor([1], device='cuda')
+    with pytest.raises(TypeError, match='float32, float16 or bfloat16'):
+        embedding(t, w)
+    with pytest.raises(TypeError, match='float32, float16 or bfloat16'):
+        embedding_grad(w[:1], t, 5)
+    with pytest.raises(TypeError, match='float32, float16 or bfloat16'):
+        token_log_probs(w[:1], t)
+    with pytest.raises(TypeError, match='float32, float16 or bfloat16'):
+        grad_norm([w])
+    with pytest.raises(ValueError, match='tokens are on'):
+        embedding(t.cpu(), w.float())
+    with pytest.raises(ValueError, match='tokens are on'):
+        token_log_probs(w[:1].float(), t.cpu())
+    with pytest.raises(RuntimeError):                          # differentiable once
+        x = w.float().requires_grad_()
+        (g,) = torch.autograd.grad(token_log_probs(x[:1], t).logprob.sum(), x, create_graph=True)
+        torch.autograd.grad(g.sum(), x)
