@@ -100,15 +100,20 @@ int mgw_embedding_grad(const void* dy, long long dy_ld, const void* tokens, int 
                        float scale, long long padding, void* dw, void* work, size_t work_bytes, int* status, void* stream);
 
 // ---- log probabilities, entropy, likeliest tokens, cross entropy (logprob.cu) -------------------------
-// stats: [rows][2] largest logit and logarithm of the sum of exp(z - it), for the backward pass (may be null).
+// stats: [rows][2] largest logit m and log2 of the sum of exp(z - m), for the backward pass (may be null).
 int mgw_logprob_fwd(const void* z, long long ld, long long rows, int vocab, int dtype, const void* tokens, int wide, long long ignore,
                     float* logprob, float* entropy, float* stats, int top, float* top_logprob, long long* top_tokens, int* status,
                     void* stream);
+// Gradient for given gradients of log probability and entropy (either may be null), or of the loss (g_loss, one value).
+// written: dz already holds the gradient for g_loss == expected (mgw_cross_entropy_fwd), nothing is done in that case.
 int mgw_logprob_bwd(const void* z, long long ld, long long rows, int vocab, int dtype, const void* tokens, int wide, long long ignore,
                     const float* stats, const float* entropy, const float* g_logprob, const float* g_entropy, const float* g_loss,
-                    const float* count, void* dz, long long dz_ld, void* stream);
-int mgw_mean_loss(const float* logprob, const void* tokens, int wide, long long ignore, long long rows, int mean, float* loss, float* count,
-                  void* stream);
+                    const int* count, int written, float expected, void* dz, long long dz_ld, void* stream);
+// Mean (or sum) of the negative log probabilities, and with dz its gradient times `expected`.  work: 2 ints, the first is
+// `count` for mgw_logprob_bwd.
+int mgw_cross_entropy_fwd(const void* z, long long ld, long long rows, int vocab, int dtype, const void* tokens, int wide,
+                          long long ignore, int mean, float expected, float* logprob, float* stats, float* loss, void* dz, long long dz_ld,
+                          int* work, int* status, void* stream);
 
 // ---- global gradient norm and clipping (grad_clip.cu) -------------------------------------------------
 // norm: 0 two-norm, 1 sum of magnitudes, 2 largest magnitude; clip = 0 only measures.  work: mgw_grad_clip_bytes(n).

@@ -16,6 +16,7 @@ On CPU tensors the same functions run plain PyTorch operations.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -35,8 +36,8 @@ def _lib_ready():
         lib = _lib.load(allow_build=False)
         p, n, i = C.c_void_p, C.c_longlong, C.c_int
         lib.mgw_logprob_fwd.argtypes = [p, n, n, i, i, p, i, n, p, p, p, i, p, p, p, p]
-        lib.mgw_logprob_bwd.argtypes = [p, n, n, i, i, p, i, n, p, p, p, p, p, p, p, n, p]
-        lib.mgw_mean_loss.argtypes = [p, p, i, n, n, i, p, p, p]
+        lib.mgw_logprob_bwd.argtypes = [p, n, n, i, i, p, i, n, p, p, p, p, p, p, i, C.c_float, p, n, p]
+        lib.mgw_cross_entropy_fwd.argtypes = [p, n, n, i, i, p, i, n, i, C.c_float, p, p, p, p, n, p, p, p]
         _ready = lib
     return _ready
 
@@ -144,7 +145,7 @@ class _TokenLogProbs(torch.autograd.Function):
             if n:
                 _lib.check(_lib_ready().mgw_logprob_bwd(z.data_ptr(), ld, n, v, DTYPE_CODES[z.dtype], tokens.data_ptr(),
                                                         tokens.dtype == torch.int64, ctx.ignore, stats.data_ptr(), h.data_ptr(), _ptr(g1),
-                                                        _ptr(g2), None, None, dz.data_ptr(), dz.stride(0) if n > 1 else v,
+                                                        _ptr(g2), None, None, 0, 0.0, dz.data_ptr(), dz.stride(0) if n > 1 else v,
                                                         stream_of(z)), 'logprob_bwd')
                 counters.bump('logprob_bwd')
             return dz.view(logits.shape), None, None, None
@@ -184,35 +185,48 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ig
 
 
 class _CrossEntropy(torch.autograd.Function):
+    """The gradient of the logits is written by the forward launch, for the gradient that the loss is expected to get: the
+    rows have just been read and come from L2.  The first backward pass hands it out (its launch looks at the actual
+    gradient and recomputes the rows only where that differs); any further one computes its own."""
+
     @staticmethod
-    def forward(ctx, logits, tokens, ignore, mean, expected_grad):
+    def forward(ctx, logits, tokens, ignore, mean, expected):
+        n, v = tokens.numel(), logits.shape[-1]
         with device_guard(logits):
             z, ld = _rows(logits)
             tokens = tokens.contiguous()
-            s = stream_of(z)
-            logprob, _, stats, _, _ = _launch_forward(z, ld, tokens, ignore, 0, False, True, s)
-            out = torch.empty(2, dtype=torch.float32, device=z.device)          # loss, number of rows it is the mean of
-            _lib.check(_lib_ready().mgw_mean_loss(logprob.data_ptr(), tokens.data_ptr(), tokens.dtype == torch.int64, ignore,
-                                                  z.shape[0], mean, out.data_ptr(), out.data_ptr() + 4, s), 'mean_loss')
-            counters.bump('mean_loss')
-        ctx.save_for_backward(logits, tokens, stats, out)
-        ctx.ignore = ignore
-        return out[0].clone()
+            train = ctx.needs_input_grad[0]
+            logprob = torch.empty(n, dtype=torch.float32, device=z.device)
+            stats = torch.empty(n, 2, dtype=torch.float32, device=z.device) if train else None
+            loss = torch.empty((), dtype=torch.float32, device=z.device)
+            work = torch.empty(2, dtype=torch.int32, device=z.device)
+            dz = _grad_like(z, ld) if train else None
+            _lib.check(_lib_ready().mgw_cross_entropy_fwd(z.data_ptr(), ld, n, v, DTYPE_CODES[z.dtype], tokens.data_ptr(),
+                                                          tokens.dtype == torch.int64, ignore, mean, expected, logprob.data_ptr(),
+                                                          _ptr(stats), loss.data_ptr(), _ptr(dz), dz.stride(0) if train and n > 1 else v,
+                                                          work.data_ptr(), status_words(), stream_of(z)), 'cross_entropy_fwd')
+            counters.bump('cross_entropy_fwd')
+        if train:
+            ctx.save_for_backward(logits, tokens, stats, work)
+            ctx.ignore, ctx.expected, ctx.dz = ignore, expected, dz
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        logits, tokens, stats, out = ctx.saved_tensors
+        logits, tokens, stats, work = ctx.saved_tensors
+        dz, ctx.dz = ctx.dz, None
+        written = dz is not None
+        n, v = tokens.numel(), logits.shape[-1]
         with device_guard(logits):
             z, ld = _rows(logits)
-            dz = _grad_like(z, ld)
-            n, v = z.shape
-            g = g.float()
+            if not written:
+                dz = _grad_like(z, ld)
             if n:
                 _lib.check(_lib_ready().mgw_logprob_bwd(z.data_ptr(), ld, n, v, DTYPE_CODES[z.dtype], tokens.data_ptr(),
                                                         tokens.dtype == torch.int64, ctx.ignore, stats.data_ptr(), None, None, None,
-                                                        g.data_ptr(), out.data_ptr() + 4, dz.data_ptr(), dz.stride(0) if n > 1 else v,
-                                                        stream_of(z)), 'cross_entropy_bwd')
+                                                        g.data_ptr(), work.data_ptr(), written, ctx.expected, dz.data_ptr(),
+                                                        dz.stride(0) if n > 1 else v, stream_of(z)), 'cross_entropy_bwd')
                 counters.bump('cross_entropy_bwd')
             return dz.view(logits.shape), None, None, None, None
 
@@ -222,8 +236,9 @@ def cross_entropy(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int 
     """Cross entropy of ``tokens`` under ``softmax(logits)`` in fp32: mean over the rows that are not padding (NaN when
     there is none, as ``torch.nn.functional.cross_entropy``), their ``'sum'``, or ``'none'``.
 
-    ``expected_grad`` is the gradient that the loss itself will get in backward (1, or the loss scale of half-precision
-    training).  Any other gradient is right too."""
+    The gradient of the logits is computed along with the loss, for the gradient that the loss itself is expected to get
+    in backward: ``expected_grad`` is 1, or the loss scale of half-precision training.  Any other gradient is right too,
+    at the cost of another pass over the logits."""
     if reduction not in ('mean', 'sum', 'none'):
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
     _check(logits, tokens)
@@ -233,7 +248,10 @@ def cross_entropy(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int 
         logprob = _reference(logits, tokens, int(ignore_index), 0)[0]
         total = -logprob.sum()
         return total / (tokens != ignore_index).sum() if reduction == 'mean' else total
-    return _CrossEntropy.apply(logits, tokens, int(ignore_index), reduction == 'mean', float(expected_grad))
+    expected = float(expected_grad)
+    if not math.isfinite(expected):
+        raise ValueError('expected_grad must be finite, got %r' % (expected_grad,))
+    return _CrossEntropy.apply(logits, tokens, int(ignore_index), reduction == 'mean', expected)
 
 
 class FusedCrossEntropyLoss(nn.CrossEntropyLoss):

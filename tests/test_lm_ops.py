@@ -230,10 +230,15 @@ def test_native_logprob_refuses_bad_arguments():
     for bad in (dict(z=None), dict(tokens=None), dict(logprob=None), dict(status=None), dict(tlp=None), dict(tt=None), dict(top=33),
                 dict(top=9), dict(top=-1), dict(vocab=0), dict(ld=7), dict(rows=-1), dict(dtype=5)):
         assert lib.mgw_logprob_fwd(*{**ok, **bad}.values()) == 2, bad
-    ok = dict(z=p, ld=8, rows=2, vocab=8, dtype=0, tokens=p, wide=0, ignore=-100, stats=p, entropy=p, g1=p, g2=p, g=None, count=None, dz=p,
-              dz_ld=8, stream=None)
-    for bad in (dict(z=None), dict(stats=None), dict(dz=None), dict(dz_ld=7), dict(entropy=None), dict(g=p)):
+    ok = dict(z=p, ld=8, rows=2, vocab=8, dtype=0, tokens=p, wide=0, ignore=-100, stats=p, entropy=p, g1=p, g2=p, g=None, count=None,
+              written=0, expected=1.0, dz=p, dz_ld=8, stream=None)
+    for bad in (dict(z=None), dict(stats=None), dict(dz=None), dict(dz_ld=7), dict(entropy=None), dict(g=p), dict(written=1)):
         assert lib.mgw_logprob_bwd(*{**ok, **bad}.values()) == 2, bad
+    ok = dict(z=p, ld=8, rows=2, vocab=8, dtype=0, tokens=p, wide=0, ignore=-100, mean=1, expected=1.0, logprob=p, stats=p, loss=p, dz=p,
+              dz_ld=8, work=p, status=p, stream=None)
+    for bad in (dict(z=None), dict(z=p + 2), dict(tokens=None), dict(logprob=None), dict(loss=None), dict(work=None), dict(status=None),
+                dict(dz_ld=7), dict(stats=p + 4), dict(vocab=0), dict(dtype=3)):
+        assert lib.mgw_cross_entropy_fwd(*{**ok, **bad}.values()) == 2, bad
 
 
 def test_native_clip_refuses_bad_arguments():
