@@ -5,8 +5,15 @@
 // Two launches and no table in device memory: the tensors' addresses and lengths travel as kernel arguments (which a
 // captured graph keeps), so nothing is uploaded and nothing has to be kept between calls.  The first launch leaves one sum
 // per block, in the second every block adds those up for itself (in a fixed order, so that all get the same factor) and
-// scales its part.  Squares are formed and added in fp64: a gradient of 1e-25 or 1e25 has a norm too, although its square
-// is no fp32 value, and the sum over hundreds of millions of values keeps its digits.
+// scales its part.  A thread adds the squares of the 16 or 32 values that it has in flight in fp32 and that sum to an
+// fp64 total, so that hundreds of millions of values keep their digits; where the values' magnitude would let squares leave
+// the range of fp32 (gradients of 1e-25 or 1e25 have a norm too), they are squared in fp64 instead.
+//
+// Both launches are bound by memory.  66 M fp32 values (264 MB): norm 41 us = 6.4 TB/s, scaling 86 us = 6.1 TB/s read and
+// written; 25.6 M values (102 MB, mostly still in L2 for the second launch): 20 + 32 us.  Squaring everything in fp64 took
+// 138 us for the norm (one block per SM: 72 registers, and a conversion for each value).  The scaling launch takes 128 us in
+// all with two blocks of 512 threads per SM, 140 with one, and 170 with three (its 63 registers a thread no longer fit);
+// stores that are marked as not read again are worth 1 %, the backward order of the second launch 2 %.
 #include <algorithm>
 #include <cstdio>
 #include <new>
@@ -19,7 +26,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kUnroll = 4;                                  // 16-byte vectors that a thread keeps in flight
 constexpr int kChunkBytes = kThreads * kUnroll * 16;        // the unit of work of a block
-constexpr int kBlocks = 148 * 4;
+constexpr int kBlocks = 148 * 3;                            // three resident blocks per SM read ...
+constexpr int kScaleBlocks = 148 * 2;                       // ... and two read and write
 
 enum { kNorm2 = 0, kNorm1 = 1, kNormMax = 2 };
 
@@ -74,6 +82,30 @@ __device__ __forceinline__ double join_values(double a, double b) {
     return !(b <= a) && a == a ? b : a;
 }
 
+// The values of one thread's vectors.  Two-norm: with the largest magnitude in (2^-40, 2^50) no sum of 32 squares
+// overflows, and what underflows is below 2^-46 of the largest square.
+template <int NORM, int N>
+__device__ __forceinline__ void add_batch(double& acc, const float (&f)[N], float most, float sum) {
+    if (NORM == kNorm2) {
+        if (most > 0x1p-40f && most < 0x1p50f) {
+            acc += (double)sum;
+            return;
+        }
+        if (most == 0.f) return;
+    } else if (NORM == kNorm1 && most < 0x1p100f) {
+        acc += (double)sum;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) add_value<NORM>(acc, f[e]);
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 template <typename T, int NORM>
 __device__ __forceinline__ void sum_piece(const Piece& p, double& acc) {
     constexpr int V = 16 / sizeof(T);
@@ -82,16 +114,25 @@ __device__ __forceinline__ void sum_piece(const Piece& p, double& acc) {
     const int vecs = (int)((p.v1 - p.v0) / V);
     uint4 r[kUnroll];
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k)
+    for (int k = 0; k < kUnroll; ++k) {
+        r[k] = make_uint4(0, 0, 0, 0);
         if (threadIdx.x + k * kThreads < vecs) r[k] = src[threadIdx.x + k * kThreads];
+    }
+    float f[kUnroll * V], most = 0.f, sum = 0.f;
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) {
-        if (threadIdx.x + k * kThreads >= vecs) continue;
-        float f[V];
-        mgw_unpack<T, V>(r[k], f);
+        float g[V];
+        mgw_unpack<T, V>(r[k], g);
 #pragma unroll
-        for (int e = 0; e < V; ++e) add_value<NORM>(acc, f[e]);
+        for (int e = 0; e < V; ++e) {
+            f[k * V + e] = g[e];
+            most = max_nan(most, fabsf(g[e]));
+            if (NORM == kNorm2) sum = fmaf(g[e], g[e], sum);
+            else if (NORM == kNorm1) sum += fabsf(g[e]);
+        }
     }
+    if (NORM == kNormMax) acc = join_values<NORM>(acc, (double)most);
+    else add_batch<NORM>(acc, f, most, sum);
     const long long head = p.v0 - p.e0, edge = head + (p.e1 - p.v1);           // fewer than 8 elements on either side
     if (threadIdx.x < edge) add_value<NORM>(acc, mgw_to_float(x[threadIdx.x < head ? p.e0 + threadIdx.x : p.v1 + threadIdx.x - head]));
 }
@@ -107,7 +148,7 @@ __device__ __forceinline__ double block_join(double v, double* red) {
 }
 
 template <int CAP, int NORM>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* __restrict__ partials) {
+__global__ void __launch_bounds__(kThreads, 3) norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* __restrict__ partials) {
     __shared__ double red[kThreads / 32];
     double acc = 0.0;
     for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
@@ -145,7 +186,7 @@ __device__ __forceinline__ void scale_piece(const Piece& p, float factor, float 
         mgw_unpack<T, V>(r[k], f);
 #pragma unroll
         for (int e = 0; e < V; ++e) f[e] = f[e] * factor * rest;
-        at[threadIdx.x + k * kThreads] = mgw_pack<T, V>(f);
+        __stcs(&at[threadIdx.x + k * kThreads], mgw_pack<T, V>(f));
     }
     const long long head = p.v0 - p.e0, edge = head + (p.e1 - p.v1);
     if (threadIdx.x < edge) {
@@ -155,7 +196,7 @@ __device__ __forceinline__ void scale_piece(const Piece& p, float factor, float 
 }
 
 template <int CAP, int NORM>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ ClipTable<CAP> t, const double* __restrict__ partials,
+__global__ void __launch_bounds__(kThreads, 2) scale_kernel(const __grid_constant__ ClipTable<CAP> t, const double* __restrict__ partials,
                                                          int n_partials, double scale, double max_norm, float* __restrict__ norm_out) {
     __shared__ double red[kThreads / 32];
     const double norm = norm_of<NORM>(partials, n_partials, scale, red);
@@ -166,8 +207,9 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
     // second a power of two (exact), so that it keeps its digits.
     const bool small = scale * c < 0x1p-100;
     const float factor = (float)(small ? scale * c * 0x1p64 : scale * c), rest = small ? 0x1p-64f : 1.f;
-    if (factor == 1.f && rest == 1.f) return;               // nothing to change
-    for (int i = blockIdx.x; i < t.chunks; i += gridDim.x) {
+    if (c == 1.0 && scale == 1.0) return;                   // a norm within the limit: nothing to change
+    // from the end: what the first launch read last is still in L2
+    for (int i = t.chunks - 1 - (int)blockIdx.x; i >= 0; i -= (int)gridDim.x) {
         const Piece p = piece_of(t, i);
         if (p.dtype == MGW_F32) scale_piece<float>(p, factor, rest);
         else if (p.dtype == MGW_F16) scale_piece<__half>(p, factor, rest);
@@ -236,7 +278,7 @@ int launch(const Call& c) {
     }
     for (int at = 0; at < c.n; at += CAP) {
         if (c.n > CAP) fill(table, c.t + at, std::min(CAP, c.n - at));
-        scale_kernel<CAP, NORM><<<std::min(kBlocks, table.chunks), kThreads, 0, c.stream>>>(table, c.partials, n_partials, c.scale, c.max_norm,
+        scale_kernel<CAP, NORM><<<std::min(kScaleBlocks, table.chunks), kThreads, 0, c.stream>>>(table, c.partials, n_partials, c.scale, c.max_norm,
                                                                                          at == 0 ? c.norm_out : nullptr);
         MGW_CUDA_CHECK(cudaGetLastError());
     }

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
 from typing import Iterable, List, Union
 
 import torch
@@ -74,15 +75,30 @@ def _check(grads: List[torch.Tensor]) -> None:
                              % (tuple(g.shape), g.stride()))
 
 
-def _launch(grads: List[torch.Tensor], code: int, scale: float, max_norm: float, clip: bool) -> torch.Tensor:
-    lib, n = _lib_ready(), len(grads)
-    with device_guard(grads[0]):
-        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
+_tensor = torch.Tensor
+
+
+def _codes(grads: List[torch.Tensor]):
+    """Type codes of the gradients when all of them are contiguous, on one GPU and of a type the kernels know, else None.
+    (Models have hundreds of gradients: five C calls for each, no Python frame.)"""
+    try:
+        codes = bytes([DTYPE_CODES[g.dtype] for g in grads])
+        if grads[0].is_cuda and len(set(map(_tensor.get_device, grads))) == 1 and all(map(_tensor.is_contiguous, grads)):
+            return codes
+    except (KeyError, RuntimeError):                      # another type; sparse
+        pass
+    return None
+
+
+def _launch(grads: List[torch.Tensor], codes: bytes, code: int, scale: float, max_norm: float, clip: bool) -> torch.Tensor:
+    lib, n, first = _lib_ready(), len(grads), grads[0]
+    ptrs, numels = array('Q', map(_tensor.data_ptr, grads)), array('q', map(_tensor.numel, grads))
+    with device_guard(first):
+        out = torch.empty((), dtype=torch.float32, device=first.device)
         need = lib.mgw_grad_clip_bytes(n)
-        work = torch.empty(need, dtype=torch.uint8, device=grads[0].device)
-        rc = lib.mgw_grad_clip((C.c_ulonglong * n)(*[g.data_ptr() for g in grads]), (C.c_longlong * n)(*[g.numel() for g in grads]),
-                               bytes(DTYPE_CODES[g.dtype] for g in grads), n, code, scale, max_norm, clip, work.data_ptr(), need,
-                               out.data_ptr(), stream_of(grads[0]))
+        work = torch.empty(need, dtype=torch.uint8, device=first.device)
+        rc = lib.mgw_grad_clip(ptrs.buffer_info()[0], numels.buffer_info()[0], codes, n, code, scale, max_norm, clip, work.data_ptr(), need,
+                               out.data_ptr(), stream_of(first))
         if rc == 2:
             raise ValueError('grad_clip: %s' % lib.mgw_last_error().decode(errors='replace'))
         _lib.check(rc, 'grad_clip')
@@ -111,10 +127,13 @@ def grad_norm(grads: Iterable[torch.Tensor], norm_type: float = 2.0, grad_scale:
     code, scale, grads = _norm_code(norm_type), _check_scale(grad_scale), list(grads)
     if not grads:
         return torch.zeros(())
-    _check(grads)
-    if not grads[0].is_cuda:
-        return _reference_norm(grads, float(norm_type), scale).float()
-    return _launch(grads, code, scale, 0.0, False)
+    codes = _codes(grads)
+    if codes is None:
+        _check(grads)
+        if not grads[0].is_cuda:
+            return _reference_norm(grads, float(norm_type), scale).float()
+        codes = bytes(DTYPE_CODES[g.dtype] for g in grads)
+    return _launch(grads, codes, code, scale, 0.0, False)
 
 
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -130,16 +149,20 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         raise ValueError('max_norm must not be negative, got %r' % (max_norm,))
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.zeros(())
-    _check(grads)
+    codes = _codes(grads)
+    if codes is None:
+        _check(grads)
+        if grads[0].is_cuda:
+            codes = bytes(DTYPE_CODES[g.dtype] for g in grads)
     if error_if_nonfinite:
         norm = grad_norm(grads, norm_type, scale)
         if not math.isfinite(float(norm)):
             raise RuntimeError('The total norm of order %s for the gradients is non-finite, so they cannot be clipped' % (norm_type,))
-    if grads[0].is_cuda:
-        return _launch(grads, code, scale, max_norm, True)
+    if codes is not None:
+        return _launch(grads, codes, code, scale, max_norm, True)
     norm = _reference_norm(grads, float(norm_type), scale)
     factor = float(scale * torch.clamp(max_norm / (norm + 1e-6), max=1.0))
     for g in {(g.data_ptr(), g.numel()): g for g in grads}.values():

@@ -21,7 +21,7 @@ import torch.nn.functional as F
 
 from . import _lib, counters
 from ._tokens import (DTYPE_CODES, TokenIndexError, check_status, check_status_nosync, check_tokens, device_guard,  # noqa: F401
-                      status_words, stream_of)
+                      once_differentiable, status_words, stream_of)
 
 _ready = None
 
@@ -127,7 +127,7 @@ class _Embedding(torch.autograd.Function):
         return _forward(tokens, weight, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dy):
         (tokens,) = ctx.saved_tensors
         return None, embedding_grad(dy, tokens, ctx.vocab, ctx.scale, ctx.padding if ctx.padding >= 0 else None), None, None

@@ -24,7 +24,7 @@ import torch.nn as nn
 
 from . import _lib, counters
 from ._tokens import (DTYPE_CODES, TokenIndexError, check_status, check_status_nosync, check_tokens, device_guard,  # noqa: F401
-                      status_words, stream_of)
+                      once_differentiable, status_words, stream_of)
 
 MAX_TOP = 32
 _ready = None
@@ -130,7 +130,7 @@ class _TokenLogProbs(torch.autograd.Function):
         return logprob, h, tlp, tt
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, g_logprob, g_entropy, _1, _2):
         logits, tokens, stats, h = ctx.saved_tensors
         if g_logprob is None and g_entropy is None:
@@ -212,7 +212,7 @@ class _CrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, g):
         logits, tokens, stats, work = ctx.saved_tensors
         dz, ctx.dz = ctx.dz, None

@@ -339,11 +339,12 @@ def test_clip_and_norm(sizes, dtypes, offset, norm_type):
             p.grad = g
         before = grad_norm(grads, norm_type, scale)
         norm = clip_grad_norm_(params, limit, norm_type, grad_scale=scale)
-        # 64-bit sums: what is left is the rounding of the norm to fp32
-        assert_within(norm, want_norm, want_norm * U * 1.01, 'norm')
+        # a thread's sum of at most 32 values is off by 32 U relatively (positive terms, one rounding each), their 64-bit
+        # total by no more, its root by half of that; then one rounding to fp32
+        assert_within(norm, want_norm, want_norm * U * (33.01 if norm_type == 1.0 else 17.01), 'norm')
         assert torch.equal(norm, before)
-        for g, w in zip(grads, want):                          # the factor and the product round in fp32, the result to the type
-            assert_within(g, w, w.abs() * (half_step(g.dtype) + 2.1 * U) + tiny(g.dtype), 'grad')
+        for g, w in zip(grads, want):                          # the norm, the factor and the product in fp32, the result in the type
+            assert_within(g, w, w.abs() * (half_step(g.dtype) + (34.1 if norm_type == 1.0 else 18.1) * U) + tiny(g.dtype), 'grad')
 
 
 def test_clip_leaves_small_gradients_alone():
@@ -400,9 +401,9 @@ def test_clip_layouts_repeats_and_overlaps():
     q.grad = torch.randn(8, 6, device='cuda').t()
     want_norm, want = _exact_clip([p.grad, q.grad], 0.5, 2.0, 1.0)
     norm = clip_grad_norm_([p, q, p, q], 0.5)                                    # each counts and is scaled once
-    assert_within(norm, want_norm, want_norm * U * 1.01, 'norm')
+    assert_within(norm, want_norm, want_norm * U * 17.01, 'norm')
     for g, w in zip((p.grad, q.grad), want):
-        assert_within(g, w, w.abs() * 3.1 * U, 'grad')
+        assert_within(g, w, w.abs() * 19.1 * U, 'grad')
     flat = torch.randn(100, device='cuda')
     a, b = torch.nn.Parameter(torch.zeros(60, device='cuda')), torch.nn.Parameter(torch.zeros(60, device='cuda'))
     a.grad, b.grad = flat[:60], flat[40:]
