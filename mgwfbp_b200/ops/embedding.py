@@ -13,6 +13,7 @@ functions run plain PyTorch operations.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
@@ -103,18 +104,28 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, num_embeddings: int
         raise TypeError('grad must be float32, float16 or bfloat16, got %s' % grad.dtype)
     if num_embeddings > 0x7ffffffe or n > 0x7fffffff:
         raise ValueError('more than 2^31 - 2 rows or 2^31 - 1 tokens')
+    return _grad_cuda(grad, tokens, num_embeddings, scale, padding)
+
+
+@functools.lru_cache(maxsize=256)
+def _work_bytes(n: int, vocab: int, dim: int, code: int) -> int:
+    return _lib_ready().mgw_embedding_grad_bytes(n, vocab, dim, code)
+
+
+def _grad_cuda(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: float, padding: int) -> torch.Tensor:
+    n, dim = tokens.numel(), grad.shape[-1]
     rows = grad.reshape(n, dim)
     if n and (rows.stride(1) != 1 or (n > 1 and rows.stride(0) < dim)):
         rows = rows.contiguous()
     tokens = tokens.contiguous()
-    lib, code = _lib_ready(), DTYPE_CODES[grad.dtype]
+    code = DTYPE_CODES[grad.dtype]
     with device_guard(grad):
-        dw = torch.empty(num_embeddings, dim, dtype=grad.dtype, device=grad.device)
-        need = lib.mgw_embedding_grad_bytes(n, num_embeddings, dim, code)
+        dw = torch.empty(vocab, dim, dtype=grad.dtype, device=grad.device)
+        need = _work_bytes(n, vocab, dim, code)
         work = torch.empty(need, dtype=torch.uint8, device=grad.device)
-        _lib.check(lib.mgw_embedding_grad(rows.data_ptr(), rows.stride(0) if n > 1 else dim, tokens.data_ptr(),
-                                          tokens.dtype == torch.int64, n, num_embeddings, dim, code, scale, padding, dw.data_ptr(),
-                                          work.data_ptr(), need, status_words(), stream_of(grad)), 'embedding_grad')
+        _lib.check(_lib_ready().mgw_embedding_grad(rows.data_ptr(), rows.stride(0) if n > 1 else dim, tokens.data_ptr(),
+                                                   tokens.dtype == torch.int64, n, vocab, dim, code, scale, padding, dw.data_ptr(),
+                                                   work.data_ptr(), need, status_words(), stream_of(grad)), 'embedding_grad')
         counters.bump('embedding_grad')
     return dw
 
@@ -130,6 +141,14 @@ class _Embedding(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         (tokens,) = ctx.saved_tensors
+        return None, _grad_cuda(dy, tokens, ctx.vocab, ctx.scale, ctx.padding), None, None
+
+
+class _EmbeddingCPU(_Embedding):
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (tokens,) = ctx.saved_tensors
         return None, embedding_grad(dy, tokens, ctx.vocab, ctx.scale, ctx.padding if ctx.padding >= 0 else None), None, None
 
 
@@ -140,7 +159,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     _check(tokens, weight)
     padding, scale = _padding(padding_idx, weight.shape[0]), float(scale)
     if torch.is_grad_enabled() and weight.requires_grad:
-        return _Embedding.apply(tokens, weight, scale, padding)
+        return (_Embedding if weight.is_cuda else _EmbeddingCPU).apply(tokens, weight, scale, padding)
     return _forward(tokens, weight, scale)
 
 

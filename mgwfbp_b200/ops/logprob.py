@@ -196,25 +196,26 @@ class _CrossEntropy(torch.autograd.Function):
             z, ld = _rows(logits)
             tokens = tokens.contiguous()
             train = ctx.needs_input_grad[0]
-            logprob = torch.empty(n, dtype=torch.float32, device=z.device)
-            stats = torch.empty(n, 2, dtype=torch.float32, device=z.device) if train else None
             loss = torch.empty((), dtype=torch.float32, device=z.device)
-            work = torch.empty(2, dtype=torch.int32, device=z.device)
+            # two words (the number of rows in the mean, a counter), {m, log2 s} of every row, log probability of every row
+            work = torch.empty(2 + 3 * n, dtype=torch.float32, device=z.device)
+            at = work.data_ptr()
             dz = _grad_like(z, ld) if train else None
             _lib.check(_lib_ready().mgw_cross_entropy_fwd(z.data_ptr(), ld, n, v, DTYPE_CODES[z.dtype], tokens.data_ptr(),
-                                                          tokens.dtype == torch.int64, ignore, mean, expected, logprob.data_ptr(),
-                                                          _ptr(stats), loss.data_ptr(), _ptr(dz), dz.stride(0) if train and n > 1 else v,
-                                                          work.data_ptr(), status_words(), stream_of(z)), 'cross_entropy_fwd')
+                                                          tokens.dtype == torch.int64, ignore, mean, expected, at + 8 + 8 * n,
+                                                          at + 8 if train else None, loss.data_ptr(), _ptr(dz),
+                                                          dz.stride(0) if train and n > 1 else v, at, status_words(), stream_of(z)),
+                       'cross_entropy_fwd')
             counters.bump('cross_entropy_fwd')
         if train:
-            ctx.save_for_backward(logits, tokens, stats, work)
+            ctx.save_for_backward(logits, tokens, work)
             ctx.ignore, ctx.expected, ctx.dz = ignore, expected, dz
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        logits, tokens, stats, work = ctx.saved_tensors
+        logits, tokens, work = ctx.saved_tensors
         dz, ctx.dz = ctx.dz, None
         written = dz is not None
         n, v = tokens.numel(), logits.shape[-1]
@@ -224,7 +225,7 @@ class _CrossEntropy(torch.autograd.Function):
                 dz = _grad_like(z, ld)
             if n:
                 _lib.check(_lib_ready().mgw_logprob_bwd(z.data_ptr(), ld, n, v, DTYPE_CODES[z.dtype], tokens.data_ptr(),
-                                                        tokens.dtype == torch.int64, ctx.ignore, stats.data_ptr(), None, None, None,
+                                                        tokens.dtype == torch.int64, ctx.ignore, work.data_ptr() + 8, None, None, None,
                                                         g.data_ptr(), work.data_ptr(), written, ctx.expected, dz.data_ptr(),
                                                         dz.stride(0) if n > 1 else v, stream_of(z)), 'cross_entropy_bwd')
                 counters.bump('cross_entropy_bwd')
