@@ -10,8 +10,12 @@
 //
 // One block reads a row once with 16-byte loads and keeps a running maximum with the sums relative to it; a row is split
 // over a cluster of up to 8 blocks when there are too few rows for all SMs, and the parts are joined through distributed
-// shared memory.  The likeliest tokens come out of the same pass: the largest value of every 32 neighbouring vectors
-// (a "group") is kept in shared memory, and only the groups with the K largest of those maxima are looked at again.
+// shared memory.  What bounds it is the number of instructions per logit, so the inner loop works on pairs: maxima and
+// the lower limit on packed bf16 or fp16, multiply-adds and sums on packed fp32.
+//
+// The likeliest tokens come out of the same pass.  Every thread knows the largest of its logits, so a value that K
+// threads reach is a lower bound for the K-th largest; every warp keeps the maximum of each 128 vectors that it read,
+// and only those that reach the bound are looked at again (from L2).  What reaches the bound is ranked by counting.
 #include <cooperative_groups.h>
 #include "api.h"
 #include "dtypes.cuh"
@@ -24,7 +28,8 @@ constexpr int kMaxTop = 32;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;                 // 16-byte vectors that a thread keeps in flight
-constexpr int kGroups = 4096;              // group maxima that a block keeps; neighbouring groups share one beyond that
+constexpr int kBatch = 32 * kUnroll;       // vectors that a warp reads at a time
+constexpr int kMaxima = 128;               // maxima that a warp keeps; neighbouring batches share one beyond that
 constexpr int kCandidates = 512;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -68,10 +73,45 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+__device__ __forceinline__ float warp_max_nan(float x) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {                // two units in the last place; 0 for very negative x
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+
+// Two fp32 values that one instruction works on.
+struct Pair { unsigned long long v; };
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ void split(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair exp2_fast(Pair p) {
+    float a, b;
+    split(p, a, b);
+    return pair(exp2_fast(a), exp2_fast(b));
 }
 
 // Whole numbers in the order of the values; NaN above everything, the two zeros equal, never 0.
@@ -80,174 +120,252 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of_key(uint32_t k) {          // NaN above plus infinity, minus infinity below its order
+    if (k <= 0x007fffffu) return -INFINITY;
+    return k >= 0xff800001u ? mgw_nan() : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
 
-// The values of a 16-byte vector, raised to `low`, and their largest before that (NaN if there is one).
+// Work on the values of a 16-byte vector in pairs.  largest(): of several vectors, NaN if there is one; values<LIFT>(): as
+// fp32, raised to `low` with LIFT; pack(): back to the type.
 template <typename T> struct Vec;
 template <> struct Vec<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ float take(const uint4& r, float (&f)[4]) {
-        f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
-        const float m = max_nan(max_nan(f[0], f[1]), max_nan(f[2], f[3]));
+    template <int K>
+    static __device__ __forceinline__ float largest(const uint4 (&r)[K]) {
+        float m = __uint_as_float(r[0].x);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = max_nan(f[e], Fast<float>::low);
+        for (int k = 0; k < K; ++k)
+            m = max_nan(max_nan(max_nan(m, __uint_as_float(r[k].x)), max_nan(__uint_as_float(r[k].y), __uint_as_float(r[k].z))),
+                        __uint_as_float(r[k].w));
         return m;
     }
+    template <bool LIFT>
+    static __device__ __forceinline__ void values(const uint4& r, Pair (&f)[2]) {
+        float a[4] = {__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z), __uint_as_float(r.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (LIFT) a[e] = max_nan(a[e], Fast<float>::low);
+        f[0] = pair(a[0], a[1]);
+        f[1] = pair(a[2], a[3]);
+    }
+    static __device__ __forceinline__ uint4 pack(const Pair (&f)[2]) {
+        uint4 r;
+        float a, b;
+        split(f[0], a, b);
+        r.x = __float_as_uint(a); r.y = __float_as_uint(b);
+        split(f[1], a, b);
+        r.z = __float_as_uint(a); r.w = __float_as_uint(b);
+        return r;
+    }
 };
+template <typename T2> __device__ __forceinline__ float2 pair_to_float(T2 h);
+template <> __device__ __forceinline__ float2 pair_to_float<__half2>(__half2 h) { return __half22float2(h); }
+template <> __device__ __forceinline__ float2 pair_to_float<__nv_bfloat162>(__nv_bfloat162 h) { return __bfloat1622float2(h); }
+template <typename T2> __device__ __forceinline__ T2 pair_from_float(float a, float b);
+template <> __device__ __forceinline__ __half2 pair_from_float<__half2>(float a, float b) { return __floats2half2_rn(a, b); }
+template <> __device__ __forceinline__ __nv_bfloat162 pair_from_float<__nv_bfloat162>(float a, float b) { return __floats2bfloat162_rn(a, b); }
+
 template <typename T, typename T2>
 struct VecHalf {
     static constexpr int N = 8;
-    static __device__ __forceinline__ float take(const uint4& r, float (&f)[8]) {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-        T2 h[4], m, low;
+    static __device__ __forceinline__ T2 word(const uint4& r, int k) {
+        const uint32_t w = k == 0 ? r.x : k == 1 ? r.y : k == 2 ? r.z : r.w;
+        return *reinterpret_cast<const T2*>(&w);
+    }
+    template <int K>
+    static __device__ __forceinline__ float largest(const uint4 (&r)[K]) {
+        T2 m = word(r[0], 0);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) m = __hmax2_nan(m, word(r[k], w));
+        const float2 f = pair_to_float(m);
+        return max_nan(f.x, f.y);
+    }
+    template <bool LIFT>
+    static __device__ __forceinline__ void values(const uint4& r, Pair (&f)[4]) {
+        T2 low;
         low.x = low.y = mgw_from_float<T>(Fast<T>::low);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) h[k] = *reinterpret_cast<const T2*>(&w[k]);
-        m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        for (int w = 0; w < 4; ++w) {
+            const float2 x = pair_to_float(LIFT ? __hmax2_nan(word(r, w), low) : word(r, w));
+            f[w] = pair(x.x, x.y);
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const Pair (&f)[4]) {
+        uint32_t w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            h[k] = __hmax2_nan(h[k], low);
-            f[2 * k] = mgw_to_float(h[k].x);
-            f[2 * k + 1] = mgw_to_float(h[k].y);
+            float a, b;
+            split(f[k], a, b);
+            const T2 h = pair_from_float<T2>(a, b);
+            w[k] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        return max_nan(mgw_to_float(m.x), mgw_to_float(m.y));
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
 template <> struct Vec<__half> : VecHalf<__half, __half2> {};
 template <> struct Vec<__nv_bfloat16> : VecHalf<__nv_bfloat16, __nv_bfloat162> {};
 
+// A thread's sums, relative to its running maximum m (in bits: M = L m).
+struct Sums {
+    float m, M;
+    Pair s, u;
+};
+
+template <bool ENT>
+__device__ __forceinline__ void raise_to(Sums& a, float m) {
+    // both products rounded, as M is everywhere: a fused subtraction would leave the rounding of the other one behind
+    const float M = __fmul_rn(m, kLog2e), d = a.M - M, f = exp2_fast(d);
+    if (ENT) a.u = mul2(pair(f, f), fma2(a.s, pair(d, d), a.u));
+    a.s = mul2(pair(f, f), a.s);
+    a.m = m;
+    a.M = M;
+}
+
+template <typename T, bool ENT>
+__device__ __forceinline__ void add_vector(Sums& a, const uint4& r) {
+    constexpr int P = Vec<T>::N / 2;
+    Pair f[P];
+    Vec<T>::template values<ENT>(r, f);                              // without u a logit of minus infinity does no harm
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+        const Pair d = fma2(f[k], pair(kLog2e, kLog2e), pair(-a.M, -a.M)), x = exp2_fast(d);
+        a.s = add2(a.s, x);
+        if (ENT) a.u = fma2(x, d, a.u);
+    }
+}
+
 struct Stats { float m, s, u; };
 
-// Sums relative to the larger maximum.
+// The block's sums: first the maximum of all, then one rescaling, then plain sums.
 template <bool ENT>
-__device__ __forceinline__ void raise_to(Stats& a, float m) {
-    // both products rounded, as M is everywhere: a fused subtraction would leave the rounding of the other one behind
-    const float d = __fmul_rn(a.m, kLog2e) - __fmul_rn(m, kLog2e), f = exp2_fast(d);
-    if (ENT) a.u = f * (a.u + a.s * d);
-    a.s *= f;
-    a.m = m;
+__device__ __forceinline__ Stats block_join(Sums x, Stats* parts) {
+    const float w = warp_max_nan(x.m);
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5].m = w;
+    __syncthreads();
+    float m = parts[0].m;
+#pragma unroll
+    for (int k = 1; k < kWarps; ++k) m = max_nan(m, parts[k].m);
+    raise_to<ENT>(x, m);
+    float s, u = 0.f, t;
+    split(x.s, s, t);
+    s += t;
+    if (ENT) {
+        split(x.u, u, t);
+        u += t;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (ENT) u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
+    if ((threadIdx.x & 31) == 0) { parts[threadIdx.x >> 5].s = s; parts[threadIdx.x >> 5].u = u; }
+    __syncthreads();
+    Stats r = {m, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+        r.s += parts[k].s;
+        if (ENT) r.u += parts[k].u;
+    }
+    return r;
 }
 
+// Two blocks' sums.
 template <bool ENT>
 __device__ __forceinline__ Stats join(Stats a, Stats b) {
-    const float m = max_nan(a.m, b.m);
-    raise_to<ENT>(a, m);
-    raise_to<ENT>(b, m);
-    a.s += b.s;
-    if (ENT) a.u += b.u;
-    return a;
-}
-
-template <bool ENT, int N>
-__device__ __forceinline__ void add_values(Stats& a, float M, const float (&f)[N]) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-        const float d = fmaf(f[e], kLog2e, -M), x = exp2_fast(d);
-        a.s += x;
-        if (ENT) a.u = fmaf(x, d, a.u);
-    }
-}
-
-template <bool ENT>
-__device__ __forceinline__ Stats block_join(Stats x, Stats* parts) {
-    for (int o = 16; o > 0; o >>= 1) {
-        Stats y;
-        y.m = __shfl_xor_sync(0xffffffffu, x.m, o);
-        y.s = __shfl_xor_sync(0xffffffffu, x.s, o);
-        y.u = ENT ? __shfl_xor_sync(0xffffffffu, x.u, o) : 0.f;
-        x = join<ENT>(x, y);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = parts[0];
-    for (int w = 1; w < kWarps; ++w) x = join<ENT>(x, parts[w]);
-    return x;
+    const float m = max_nan(a.m, b.m), M = __fmul_rn(m, kLog2e);
+    const float da = __fmul_rn(a.m, kLog2e) - M, db = __fmul_rn(b.m, kLog2e) - M, fa = exp2_fast(da), fb = exp2_fast(db);
+    Stats r = {m, a.s * fa + b.s * fb, 0.f};
+    if (ENT) r.u = fa * (a.u + a.s * da) + fb * (b.u + b.s * db);
+    return r;
 }
 
 // ------------------------------------------------------------------------------------------------ layout of a row
-// Elements before the first 16-byte boundary (head), whole vectors, elements behind them (tail).  Groups: 0 the head,
-// then 32 vectors each, the last one the tail; a block of a cluster has groups [g0, g1).
+// Elements before the first 16-byte boundary (head), whole vectors, elements behind them (tail).  A block of a cluster
+// has the vectors [v0, v1); the first block also has the head, the last one the tail.
 template <typename T>
 struct Row {
     const T* z;
-    int head, n_vec, tail0, vocab, groups;
-    __device__ __forceinline__ Row(const T* z_, int vocab_) : z(z_), vocab(vocab_) {
+    int head, n_vec, tail0, vocab, v0, v1;
+    bool has_head, has_tail;
+    __device__ __forceinline__ Row(const T* z_, int vocab_, int part, int splits) : z(z_), vocab(vocab_) {
         const int h = (int)(((16 - ((unsigned long long)z_ & 15)) & 15) / sizeof(T));
         head = min(h, vocab_);
         n_vec = (vocab_ - head) / Vec<T>::N;
         tail0 = head + n_vec * Vec<T>::N;
-        groups = ((n_vec + 31) >> 5) + 2;
+        const int per = splits == 1 ? n_vec : (((n_vec + splits - 1) / splits + 31) & ~31);
+        v0 = (int)min((long long)n_vec, (long long)part * per);
+        v1 = (int)min((long long)n_vec, (long long)v0 + per);
+        has_head = part == 0;
+        has_tail = part == splits - 1;
     }
     __device__ __forceinline__ uint4 vec(int i) const { return reinterpret_cast<const uint4*>(z + head)[i]; }
+    // the element at the edge that a thread of the block looks after (0 .. 15), or -1
+    __device__ __forceinline__ int edge(int thread) const {
+        if (thread < 8) return has_head && thread < head ? thread : -1;
+        return thread < 16 && has_tail && tail0 + thread - 8 < vocab ? tail0 + thread - 8 : -1;
+    }
 };
 
-// Sums and group maxima of this block's groups.
+struct TopSpace {
+    float maxima[kWarps][kMaxima];         // of the batches of a warp
+    uint32_t most[kThreads];               // order of the threads' maxima, 0: the thread has no vector
+    uint32_t floor;                        // a lower bound of the order of the K-th largest value
+    unsigned long long list[kWarps][32];
+    unsigned long long candidate[kCandidates];
+    int n_candidates;
+};
+
+// Sums of this block's part of the row; with TOP also the batches' maxima and the thread's own (most: minus infinity
+// where it has no vector).
 template <typename T, bool ENT, bool TOP>
-__device__ __forceinline__ Stats scan_row(const Row<T>& row, int g0, int g1, int shift, uint32_t* group_key) {
-    constexpr int N = Vec<T>::N;
+__device__ __forceinline__ Sums scan_row(const Row<T>& row, int shift, TopSpace* top, float& most) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Stats a = {Fast<T>::start, 0.f, 0.f};
-    float M = a.m * kLog2e;
-    const int b0 = max(g0, 1), b1 = min(g1, row.groups - 1);         // the groups of vectors among them
-    for (int g = b0 + warp; g < b1; g += kWarps * kUnroll) {
-        uint4 r[kUnroll];
+    Sums a;
+    a.m = Fast<T>::start;
+    a.M = __fmul_rn(a.m, kLog2e);
+    a.s = a.u = pair(0.f, 0.f);
+    most = -INFINITY;
+    int batch = 0;
+    for (int i0 = row.v0 + warp * kBatch; i0 < row.v1; i0 += kWarps * kBatch, ++batch) {
+        float m;
+        if (i0 + kBatch <= row.v1) {
+            uint4 r[kUnroll];
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            const int i = (g + k * kWarps - 1) * 32 + lane;
-            if (g + k * kWarps < b1 && i < row.n_vec) r[k] = row.vec(i);
-        }
-        float f[kUnroll][N], top[kUnroll], most = Fast<T>::start;
+            for (int k = 0; k < kUnroll; ++k) r[k] = row.vec(i0 + k * 32 + lane);
+            m = Vec<T>::largest(r);
+            const float up = max_nan(a.m, m);
+            if (up != a.m) raise_to<ENT>(a, up);
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            const bool in = g + k * kWarps < b1 && (g + k * kWarps - 1) * 32 + lane < row.n_vec;
-            if (in) {
-                top[k] = Vec<T>::take(r[k], f[k]);
-                most = max_nan(most, top[k]);
-            } else {
-                top[k] = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < N; ++e) f[k][e] = Fast<T>::low;
-            }
-            if (TOP && g + k * kWarps < b1) {
-                const uint32_t key = __reduce_max_sync(0xffffffffu, in ? order_key(top[k]) : 0u);
-                if (lane == 0) {
-                    if (shift == 0) group_key[g + k * kWarps - g0] = key;
-                    else atomicMax(&group_key[(g + k * kWarps - g0) >> shift], key);
-                }
+            for (int k = 0; k < kUnroll; ++k) add_vector<T, ENT>(a, r[k]);
+        } else {                                                     // the last batch of the part
+            m = -INFINITY;
+            for (int i = i0 + lane; i < row.v1; i += 32) {
+                const uint4 r[1] = {row.vec(i)};
+                m = max_nan(m, Vec<T>::largest(r));
+                const float up = max_nan(a.m, m);
+                if (up != a.m) raise_to<ENT>(a, up);
+                add_vector<T, ENT>(a, r[0]);
             }
         }
-        const float m = max_nan(a.m, most);
-        if (m != a.m) {
-            raise_to<ENT>(a, m);
-            M = m * kLog2e;
+        if (TOP) {
+            most = max_nan(most, m);
+            const float w = warp_max_nan(m);
+            if (lane == 0) {
+                float* to = &top->maxima[warp][batch >> shift];
+                *to = (batch & ((1 << shift) - 1)) == 0 ? w : max_nan(*to, w);
+            }
         }
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k)
-            if (g + k * kWarps < b1 && (g + k * kWarps - 1) * 32 + lane < row.n_vec) add_values<ENT, N>(a, M, f[k]);
     }
-    // the few elements of head and tail: one per lane of the first warp
-    if (warp == 0) {
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            const int g = side == 0 ? 0 : row.groups - 1;
-            if (g < g0 || g >= g1) continue;
-            const int j = side == 0 ? lane : row.tail0 + lane;
-            const bool in = j < (side == 0 ? row.head : row.vocab);
-            const float v = in ? mgw_to_float(row.z[j]) : -INFINITY;
-            if (TOP) {
-                const uint32_t key = __reduce_max_sync(0xffffffffu, in ? order_key(v) : 0u);
-                if (lane == 0) {
-                    if (shift == 0) group_key[g - g0] = key;
-                    else atomicMax(&group_key[(g - g0) >> shift], key);
-                }
-            }
-            if (in) {
-                const float m = max_nan(a.m, v);
-                if (m != a.m) raise_to<ENT>(a, m);
-                const float f[1] = {max_nan(v, Fast<T>::low)};
-                add_values<ENT, 1>(a, a.m * kLog2e, f);
-            }
-        }
+    const int j = row.edge(threadIdx.x);
+    if (j >= 0) {
+        const float v = mgw_to_float(row.z[j]);
+        const float up = max_nan(a.m, v);
+        if (up != a.m) raise_to<ENT>(a, up);
+        const float d = fmaf(max_nan(v, Fast<T>::low), kLog2e, -a.M), x = exp2_fast(d);
+        a.s = add2(a.s, pair(x, 0.f));
+        if (ENT) a.u = fma2(pair(x, 0.f), pair(d, 0.f), a.u);
     }
     return a;
 }
@@ -255,10 +373,10 @@ __device__ __forceinline__ Stats scan_row(const Row<T>& row, int g0, int g1, int
 // A row whose maximum is at the edge of the type's range: differences first, minus infinity left out.  m may end up
 // infinite or NaN; s and u are relative to m, u in bits.
 template <typename T>
-__device__ Stats careful_row(const T* z, int vocab, Stats* parts) {
+__device__ __noinline__ Stats careful_row(const T* z, int vocab, Stats* parts) {
     float m = -INFINITY;
     for (int j = threadIdx.x; j < vocab; j += kThreads) m = max_nan(m, mgw_to_float(z[j]));
-    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = warp_max_nan(m);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5].m = m;
     __syncthreads();
@@ -296,8 +414,8 @@ __device__ __forceinline__ float ln_prob(float v, float m, float log2_s) {
 }
 
 // -------------------------------------------------------------------------------------------------- likeliest tokens
-// A warp's list: the 32 largest keys seen so far, one per lane, largest first.  A key is the value's order and below
-// it the complement of the index, so equal values are ordered by the lower index and no two keys are equal; 0 is none.
+// A key is the value's order and below it the complement of the index, so equal values are ordered by the lower index
+// and no two keys are equal; 0 is none.
 typedef unsigned long long Key;
 
 __device__ __forceinline__ Key key_of(float v, int index) { return ((Key)order_key(v) << 32) | (0xffffffffu - (uint32_t)index); }
@@ -327,173 +445,187 @@ __device__ __forceinline__ Key merge_lists(Key a, Key b) {           // both des
     return x;
 }
 
-struct TopSpace {
-    uint32_t group_key[kGroups];
-    Key list[kWarps][32];
-    Key chosen[32];                        // the groups to look at again, by their maxima
-    Key candidate[kCandidates];
-    int n_candidates;
-};
-
-// The warps' lists become one, in the first warp.
-__device__ __forceinline__ Key join_lists(Key mine, TopSpace* t) {
+// Many equal or rising values: every warp keeps a sorted list of the 32 largest and goes through its part of the row, 32
+// values at a time.  The `top` largest keys end up in t->candidate.
+template <typename T>
+__device__ __noinline__ int top_by_lists(const Row<T>& row, int top, float floor, TopSpace* t) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Key mine = 0;
+    auto offer = [&](Key x) {
+        const Key least = __shfl_sync(0xffffffffu, mine, 31);
+        if (__any_sync(0xffffffffu, x > least)) mine = merge_lists(mine, sort_lanes(x));
+    };
+    for (int i0 = row.v0 + warp * 32; i0 < row.v1; i0 += kWarps * 32) {
+        const bool in = i0 + lane < row.v1;
+        float f[Vec<T>::N];
+        if (in) mgw_unpack<T, Vec<T>::N>(row.vec(i0 + lane), f);
+#pragma unroll
+        for (int e = 0; e < Vec<T>::N; ++e)
+            offer(in && !(f[e] < floor) ? key_of(f[e], row.head + (i0 + lane) * Vec<T>::N + e) : (Key)0);
+    }
+    if (warp == 0) {
+        const int j = row.edge(lane);
+        offer(j >= 0 ? key_of(mgw_to_float(row.z[j]), j) : (Key)0);
+    }
     t->list[warp][lane] = mine;
     __syncthreads();
-    if (warp == 0)
-        for (int w = 1; w < kWarps; ++w)
-            if (t->list[w][0] != 0) mine = merge_lists(mine, t->list[w][lane]);
-    return mine;
-}
-
-// The elements of a group (of 2^shift neighbouring groups), one call of `use` per vector element and all lanes at once.
-template <typename T, typename F>
-__device__ __forceinline__ void for_group(const Row<T>& row, int local, int g0, int g1, int shift, F use) {
-    const int lane = threadIdx.x & 31;
-    const int from = g0 + (local << shift), to = min(g1, from + (1 << shift));
-    for (int g = from; g < to; ++g) {
-        if (g == 0 || g == row.groups - 1) {
-            const int j = g == 0 ? lane : row.tail0 + lane;
-            const bool in = j < (g == 0 ? row.head : row.vocab);
-            use(in ? key_of(mgw_to_float(row.z[j]), j) : (Key)0);
-            continue;
-        }
-        const int i = (g - 1) * 32 + lane;
-        const bool in = i < row.n_vec;
-        float f[Vec<T>::N];
-        if (in) mgw_unpack<T, Vec<T>::N>(row.vec(i), f);
-#pragma unroll
-        for (int e = 0; e < Vec<T>::N; ++e) use(in ? key_of(f[e], row.head + i * Vec<T>::N + e) : (Key)0);
+    if (warp == 0) {
+        for (int w = 1; w < kWarps; ++w) mine = merge_lists(mine, t->list[w][lane]);
+        if (lane < top) t->candidate[lane] = mine;
     }
+    __syncthreads();
+    return top;
 }
 
-// The largest keys of this block's groups, in the first warp (other warps return nothing of use).
+// Keys that hold the `top` largest of this block's part of the row: t->candidate[0 .. returned).
 template <typename T>
-__device__ Key top_of_block(const Row<T>& row, int g0, int g1, int shift, int top, TopSpace* t) {
+__device__ __forceinline__ int find_candidates(const Row<T>& row, int top, int shift, float most, TopSpace* t) {
+    constexpr int N = Vec<T>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n = (g1 - g0 + (1 << shift) - 1) >> shift;
-    Key mine = 0;
-    for (int at = warp * 32; at < n; at += kThreads) {
-        const Key k = at + lane < n && t->group_key[at + lane] != 0
-                          ? ((Key)t->group_key[at + lane] << 32) | (0xffffffffu - (uint32_t)(at + lane)) : (Key)0;
-        mine = merge_lists(mine, sort_lanes(k));
-    }
-    mine = join_lists(mine, t);
-    if (warp == 0) t->chosen[lane] = lane < top ? mine : (Key)0;
+    // the bound: a value that `top` of the threads' maxima reach, found bit by bit (the upper 16 bits of the order) by one warp
+    t->most[threadIdx.x] = row.v0 + warp * kBatch + lane < row.v1 ? order_key(most) : 0u;
     if (threadIdx.x == 0) t->n_candidates = 0;
     __syncthreads();
-    // every wanted element is in one of these groups and not below the smallest of their maxima
-    const uint32_t floor_key = (uint32_t)(t->chosen[top - 1] >> 32);
-    for (int k = warp; k < top; k += kWarps) {
-        const Key c = t->chosen[k];
-        if (c == 0) break;
-        for_group(row, (int)(0xffffffffu - (uint32_t)c), g0, g1, shift, [&](Key x) {
-            const bool good = x != 0 && (uint32_t)(x >> 32) >= floor_key;
-            const unsigned who = __ballot_sync(0xffffffffu, good);
-            if (who == 0) return;
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&t->n_candidates, __popc(who));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-            if (good && at < kCandidates) t->candidate[at] = x;
-        });
+    if (warp == 0) {
+        uint32_t key[kWarps], bound = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) key[w] = t->most[w * 32 + lane];
+#pragma unroll
+        for (int bit = 31; bit >= 16; --bit) {
+            const uint32_t next = bound | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) n += key[w] >= next;
+            if (__reduce_add_sync(0xffffffffu, n) >= top) bound = next;
+        }
+        if (lane == 0) t->floor = bound;
     }
     __syncthreads();
-    mine = 0;
-    const int found = t->n_candidates;
-    if (found <= kCandidates) {                                      // their order does not matter: keys are unique
-        if (found <= 64) {
-            if (warp == 0)
-                for (int at = 0; at < found; at += 32) mine = merge_lists(mine, sort_lanes(at + lane < found ? t->candidate[at + lane] : (Key)0));
-            return mine;
-        }
-        for (int at = warp * 32; at < found; at += kThreads)
-            mine = merge_lists(mine, sort_lanes(at + lane < found ? t->candidate[at + lane] : (Key)0));
-    } else {                                                         // many equal or rising values: go through the groups
-        for (int k = warp; k < top; k += kWarps) {
-            const Key c = t->chosen[k];
-            if (c == 0) break;
-            for_group(row, (int)(0xffffffffu - (uint32_t)c), g0, g1, shift, [&](Key x) {
-                const Key least = __shfl_sync(0xffffffffu, mine, 31);
-                if (__any_sync(0xffffffffu, x > least)) mine = merge_lists(mine, sort_lanes(x));
-            });
+    const uint32_t low = t->floor;
+    const float floor = value_of_key(low);
+    auto take = [&](float v, int j) {
+        const int at = atomicAdd(&t->n_candidates, 1);               // their order does not matter: they are ranked
+        if (at < kCandidates) t->candidate[at] = key_of(v, j);
+    };
+    int batch = 0;
+    for (int i0 = row.v0 + warp * kBatch; i0 < row.v1; i0 += kWarps * kBatch, ++batch) {
+        if (t->maxima[warp][batch >> shift] < floor) continue;
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            const int i = i0 + k * 32 + lane;
+            if (i >= row.v1) continue;
+            const uint4 r[1] = {row.vec(i)};
+            if (Vec<T>::largest(r) < floor) continue;
+            float f[N];
+            mgw_unpack<T, N>(r[0], f);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (!(f[e] < floor)) take(f[e], row.head + i * N + e);
         }
     }
-    return join_lists(mine, t);
+    const int j = row.edge(threadIdx.x);
+    if (j >= 0) {
+        const float v = mgw_to_float(row.z[j]);
+        if (!(v < floor)) take(v, j);
+    }
+    __syncthreads();
+    const int found = t->n_candidates;
+    return found <= kCandidates ? found : top_by_lists(row, top, floor, t);
 }
 
-// ------------------------------------------------------------------------------------------------------------ forward
-// One row (the columns of groups [g0, g1)) of a gradient: value(logit, column).  Whole vectors where logits and gradient
-// start at the same place of a 16-byte block, single elements otherwise.  READ: the logits are needed.
-template <typename T, bool READ, typename F>
-__device__ __forceinline__ void write_row(const Row<T>& row, T* dz, int g0, int g1, F value) {
+// How many of n keys are larger.
+__device__ __forceinline__ int rank_of(Key x, const Key* keys, int n) {
+    int r = 0;
+    for (int i = 0; i < n; ++i) r += keys[i] > x;
+    return r;
+}
+
+// ------------------------------------------------------------------------------------------- gradient of one row
+// The block's part of a row of a gradient.  pairs(Pair logits) and one(logit, column) give the values; the column `t` is
+// always done by one().  Whole vectors where logits and gradient start at the same place of a 16-byte block.
+template <typename T, bool READ, bool LIFT, typename FP, typename F1>
+__device__ __forceinline__ void write_row(const Row<T>& row, T* dz, long long t, FP pairs, F1 one) {
     constexpr int N = Vec<T>::N;
-    const int v0 = (max(g0, 1) - 1) * 32, v1 = min(row.n_vec, (min(g1, row.groups - 1) - 1) * 32);
     if (((unsigned long long)dz & 15) == ((unsigned long long)row.z & 15)) {
         uint4* to = reinterpret_cast<uint4*>(dz + row.head);
-        for (int i0 = v0 + threadIdx.x; i0 < v1; i0 += kThreads * kUnroll) {
-            uint4 q[kUnroll];
+        const int ti = t >= row.head && t < row.tail0 ? ((int)t - row.head) / N : -1;      // the vector with column t
+        auto finish = [&](const uint4& q, int i) {
+            Pair f[N / 2];
+            if (READ) Vec<T>::template values<LIFT>(q, f);
 #pragma unroll
-            for (int k = 0; k < kUnroll; ++k)
-                if (READ && i0 + k * kThreads < v1) q[k] = row.vec(i0 + k * kThreads);
+            for (int k = 0; k < N / 2; ++k) f[k] = pairs(f[k]);
+            to[i] = Vec<T>::pack(f);
+            if (i == ti) dz[t] = mgw_from_float<T>(one(READ ? mgw_to_float(row.z[t]) : 0.f, (int)t));
+        };
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        for (int i0 = row.v0 + warp * kBatch; i0 < row.v1; i0 += kWarps * kBatch) {
+            if (i0 + kBatch <= row.v1) {
+                uint4 q[kUnroll];
 #pragma unroll
-            for (int k = 0; k < kUnroll; ++k) {
-                const int i = i0 + k * kThreads;
-                if (i >= v1) continue;
-                float f[N];
-                if (READ) mgw_unpack<T, N>(q[k], f);
+                for (int k = 0; k < kUnroll; ++k)
+                    if (READ) q[k] = row.vec(i0 + k * 32 + lane);
 #pragma unroll
-                for (int e = 0; e < N; ++e) f[e] = value(READ ? f[e] : 0.f, row.head + i * N + e);
-                to[i] = mgw_pack<T, N>(f);
+                for (int k = 0; k < kUnroll; ++k) finish(q[k], i0 + k * 32 + lane);
+            } else {
+                for (int i = i0 + lane; i < row.v1; i += 32) {
+                    uint4 q;
+                    if (READ) q = row.vec(i);
+                    finish(q, i);
+                }
             }
         }
     } else {
-        for (int j = row.head + v0 * N + threadIdx.x; j < row.head + v1 * N; j += kThreads)
-            dz[j] = mgw_from_float<T>(value(READ ? mgw_to_float(row.z[j]) : 0.f, j));
+        for (int j = row.head + row.v0 * N + threadIdx.x; j < row.head + row.v1 * N; j += kThreads)
+            dz[j] = mgw_from_float<T>(one(READ ? mgw_to_float(row.z[j]) : 0.f, j));
     }
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-        const int g = side == 0 ? 0 : row.groups - 1, j = (side == 0 ? 0 : row.tail0) + threadIdx.x;
-        if (g >= g0 && g < g1 && j < (side == 0 ? row.head : row.vocab))
-            dz[j] = mgw_from_float<T>(value(READ ? mgw_to_float(row.z[j]) : 0.f, j));
+    const int j = row.edge(threadIdx.x);
+    if (j >= 0) dz[j] = mgw_from_float<T>(one(READ ? mgw_to_float(row.z[j]) : 0.f, j));
+}
+
+template <typename T>
+__device__ __noinline__ void write_constant(const Row<T>& row, T* dz, float c) {
+    write_row<T, false, false>(row, dz, -1, [=](Pair) { return pair(c, c); }, [=](float, int) { return c; });
+}
+
+// A row whose maximum is at the edge of the range: -p (base + slope log2 p) + g1 delta, one by one.
+template <typename T>
+__device__ __noinline__ void write_careful(const Row<T>& row, T* dz, float m, float log2_s, float base, float slope, float g1, long long t) {
+    const int j0 = row.has_head ? 0 : row.head + row.v0 * Vec<T>::N, j1 = row.has_tail ? row.vocab : row.head + row.v1 * Vec<T>::N;
+    for (int j = j0 + threadIdx.x; j < j1; j += kThreads) {
+        const float d = fmaxf((mgw_to_float(row.z[j]) - m) * kLog2e - log2_s, -1e4f);      // p = 0 well before
+        const float x = -exp2_fast(d) * fmaf(slope, d, base);
+        dz[j] = mgw_from_float<T>(j == t ? x + g1 : x);
     }
 }
 
-// g (p - delta), the gradient of one row's loss
+// g (p - delta), the gradient of one row's loss: 2^(L z - M) times g / s
 template <typename T>
-__device__ __forceinline__ void write_loss_gradient(const Row<T>& row, T* dz, int g0, int g1, float m, float log2_s, float g, long long t) {
+__device__ __forceinline__ void write_loss_gradient(const Row<T>& row, T* dz, float m, float log2_s, float g, long long t) {
     if (careful<T>(m)) {
-        write_row<T, true>(row, dz, g0, g1, [=](float v, int j) {
-            const float p = exp2_fast(log2_prob<T>(v, m, log2_s));
-            return g * (j == t ? p - 1.f : p);
-        });
+        write_careful(row, dz, m, log2_s, -g, 0.f, -g, t);
         return;
     }
-    const float M = m * kLog2e;
-    write_row<T, true>(row, dz, g0, g1, [=](float v, int j) {
-        const float p = exp2_fast(fmaf(v, kLog2e, -M) - log2_s);
-        return g * (j == t ? p - 1.f : p);
-    });
+    const float M = __fmul_rn(m, kLog2e), gs = g * exp2f(-log2_s);
+    write_row<T, true, false>(
+        row, dz, t, [=](Pair v) { return mul2(exp2_fast(fma2(v, pair(kLog2e, kLog2e), pair(-M, -M))), pair(gs, gs)); },
+        [=](float v, int j) {
+            const float x = exp2_fast(fmaf(v, kLog2e, -M)) * gs;
+            return j == t ? x - g : x;
+        });
 }
 
-template <typename T>
-__device__ __forceinline__ void write_constant(const Row<T>& row, T* dz, int g0, int g1, float c) {
-    write_row<T, false>(row, dz, g0, g1, [=](float, int) { return c; });
-}
-
+// ------------------------------------------------------------------------------------------------------------ forward
 template <typename T, bool ENT, bool TOP, bool LOSS>
-__global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(RowArgs a) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     TopSpace* top = reinterpret_cast<TopSpace*>(dynamic);            // only with TOP
     __shared__ Stats parts[kWarps];
     __shared__ Stats of_block;
-    __shared__ Key block_list[32];
-    const int part = blockIdx.x % a.splits;
-    const long long r = blockIdx.x / a.splits;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ Key block_list[kMaxTop];
+    const int part = a.splits == 1 ? 0 : blockIdx.x % a.splits;
+    const long long r = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
     const long long t = mgw_token(a.tokens, a.wide, r);
-    const Row<T> row(static_cast<const T*>(a.z) + r * a.ld, a.vocab);
-    const int per = (row.groups + a.splits - 1) / a.splits;
-    const int g0 = min(row.groups, part * per), g1 = min(row.groups, g0 + per);
+    const Row<T> row(static_cast<const T*>(a.z) + r * a.ld, a.vocab, part, a.splits);
     if (t == a.ignore) {                                             // all blocks of the cluster leave
         if (part == 0) {
             if (threadIdx.x == 0) {
@@ -507,17 +639,13 @@ __global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(RowArgs a) {
                     a.top_tokens[r * a.top + k] = -1;
                 }
         }
-        if (LOSS && a.dz != nullptr) write_constant(row, static_cast<T*>(a.dz) + r * a.dz_ld, g0, g1, 0.f);
+        if (LOSS && a.dz != nullptr) write_constant(row, static_cast<T*>(a.dz) + r * a.dz_ld, 0.f);
     } else {
         int shift = 0;
-        if (TOP) {
-            while (((g1 - g0) >> shift) >= kGroups) ++shift;
-            if (shift > 0) {
-                for (int k = threadIdx.x; k < kGroups; k += kThreads) top->group_key[k] = 0;
-                __syncthreads();
-            }
-        }
-        Stats x = block_join<ENT>(scan_row<T, ENT, TOP>(row, g0, g1, shift, top->group_key), parts);
+        if (TOP)
+            while (((row.v1 - row.v0) / (kWarps * kBatch) >> shift) >= kMaxima) ++shift;
+        float most;
+        Stats x = block_join<ENT>(scan_row<T, ENT, TOP>(row, shift, top, most), parts);
         if (a.splits > 1) {
             cg::cluster_group cluster = cg::this_cluster();
             if (threadIdx.x == 0) of_block = x;
@@ -536,24 +664,36 @@ __global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(RowArgs a) {
             if (a.stats) a.stats[r] = make_float2(fine ? x.m : mgw_nan(), log2_s);
         }
         if (TOP) {
-            Key mine = top_of_block(row, g0, g1, shift, a.top, top);
-            if (a.splits > 1) {
+            int n = find_candidates(row, a.top, shift, most, top);
+            const Key* from = top->candidate;
+            if (a.splits > 1) {                                      // every block's `top` largest, then those of all
                 cg::cluster_group cluster = cg::this_cluster();
-                if (warp == 0) block_list[lane] = mine;
+                if (threadIdx.x < kMaxTop) block_list[threadIdx.x] = 0;
+                __syncthreads();
+                for (int i = threadIdx.x; i < n; i += kThreads) {
+                    const int k = rank_of(from[i], from, n);
+                    if (k < a.top) block_list[k] = from[i];
+                }
                 cluster.sync();
-                if (part == 0 && warp == 0)
-                    for (int k = 1; k < a.splits; ++k) mine = merge_lists(mine, *cluster.map_shared_rank(&block_list[lane], k));
+                n = a.splits * a.top;
+                if (part == 0)
+                    for (int i = threadIdx.x; i < n; i += kThreads) top->candidate[i] = *cluster.map_shared_rank(&block_list[i % a.top], i / a.top);
+                __syncthreads();
             }
-            if (part == 0 && warp == 0 && lane < a.top) {
-                const int j = (int)(0xffffffffu - (uint32_t)mine);
-                a.top_tokens[r * a.top + lane] = j;
-                a.top_logprob[r * a.top + lane] = fine ? ln_prob<T>(mgw_to_float(row.z[j]), x.m, log2_s) : mgw_nan();
-            }
+            if (part == 0)
+                for (int i = threadIdx.x; i < n; i += kThreads) {
+                    const Key key = from[i];
+                    const int k = key != 0 ? rank_of(key, from, n) : a.top;
+                    if (k >= a.top) continue;
+                    const int j = (int)(0xffffffffu - (uint32_t)key);
+                    a.top_tokens[r * a.top + k] = j;
+                    a.top_logprob[r * a.top + k] = fine ? ln_prob<T>(mgw_to_float(row.z[j]), x.m, log2_s) : mgw_nan();
+                }
         }
         if (LOSS && a.dz != nullptr) {                               // the row was just read: it comes from L2
             T* dz = static_cast<T*>(a.dz) + r * a.dz_ld;
-            if (fine && valid) write_loss_gradient(row, dz, g0, g1, x.m, log2_s, a.expected / (float)*a.count, t);
-            else write_constant(row, dz, g0, g1, mgw_nan());
+            if (fine && valid) write_loss_gradient(row, dz, x.m, log2_s, a.expected / (float)*a.count, t);
+            else write_constant(row, dz, mgw_nan());
         }
         if (a.splits > 1) cg::this_cluster().sync();                 // until here the others may read this block's memory
     }
@@ -561,6 +701,7 @@ __global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(RowArgs a) {
         // the block that finishes last adds up the rows: thread i rows i, i + 256, ..., the same order every time
         __shared__ bool last;
         __shared__ double sums[kWarps];
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         if (threadIdx.x == 0) {
             __threadfence();
             last = atomicAdd(a.done, 1u) == (unsigned)(a.rows - 1);
@@ -621,39 +762,47 @@ struct GradArgs {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(GradArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(GradArgs a) {
     const float g_loss = a.g_loss != nullptr ? *a.g_loss : 0.f;
     if (a.written && g_loss == a.expected) return;
     for (long long task = blockIdx.x; task < a.rows * a.splits; task += gridDim.x) {
-        const long long r = task / a.splits;
+        const long long r = a.splits == 1 ? task : task / a.splits;
         const int part = (int)(task - r * a.splits);
         const long long t = mgw_token(a.tokens, a.wide, r);
-        const Row<T> row(static_cast<const T*>(a.z) + r * a.ld, a.vocab);
+        const Row<T> row(static_cast<const T*>(a.z) + r * a.ld, a.vocab, part, a.splits);
         T* dz = static_cast<T*>(a.dz) + r * a.dz_ld;
-        const int per = (row.groups + a.splits - 1) / a.splits;
-        const int g0 = min(row.groups, part * per), g1 = min(row.groups, g0 + per);
         if (t == a.ignore) {
-            write_constant(row, dz, g0, g1, 0.f);
+            write_constant(row, dz, 0.f);
             continue;
         }
         const float m = a.stats[r].x, log2_s = a.stats[r].y;
         if (t < 0 || t >= a.vocab || m != m) {
-            write_constant(row, dz, g0, g1, mgw_nan());
+            write_constant(row, dz, mgw_nan());
             continue;
         }
         if (a.g_loss != nullptr) {
-            write_loss_gradient(row, dz, g0, g1, m, log2_s, g_loss / (float)*a.count, t);
+            write_loss_gradient(row, dz, m, log2_s, g_loss / (float)*a.count, t);
             continue;
         }
-        // g1 (delta - p) - g2 p (ln p + H)
-        const float h = a.entropy ? a.entropy[r] : 0.f, g1v = a.g_logprob ? a.g_logprob[r] : 0.f, g2 = a.g_entropy ? a.g_entropy[r] : 0.f;
-        const float base = g1v + g2 * h, slope = g2 * kLn2, M = m * kLog2e;
-        const bool edge = careful<T>(m);
-        write_row<T, true>(row, dz, g0, g1, [=](float v, int j) {
-            const float d = fmaxf((edge ? (v - m) * kLog2e : fmaf(v, kLog2e, -M)) - log2_s, -1e4f);      // p = 0 well before
-            const float x = -exp2_fast(d) * fmaf(slope, d, base);
-            return j == t ? x + g1v : x;
-        });
+        // g1 (delta - p) - g2 p (ln p + H); with d = L z - M:  p = 2^d / s,  ln p = ln 2 (d - log2 s)
+        const float h = a.entropy ? a.entropy[r] : 0.f, g1 = a.g_logprob ? a.g_logprob[r] : 0.f, g2 = a.g_entropy ? a.g_entropy[r] : 0.f;
+        const float slope = g2 * kLn2, M = __fmul_rn(m, kLog2e);
+        if (careful<T>(m)) {
+            write_careful(row, dz, m, log2_s, g1 + g2 * h, slope, g1, t);
+            continue;
+        }
+        const float base = g1 + g2 * h - slope * log2_s, rs = -exp2f(-log2_s);
+        write_row<T, true, true>(
+            row, dz, t,
+            [=](Pair v) {
+                const Pair d = fma2(v, pair(kLog2e, kLog2e), pair(-M, -M));
+                return mul2(mul2(exp2_fast(d), pair(rs, rs)), fma2(pair(slope, slope), d, pair(base, base)));
+            },
+            [=](float v, int j) {
+                const float d = fmaf(max_nan(v, Fast<T>::low), kLog2e, -M);
+                const float x = exp2_fast(d) * rs * fmaf(slope, d, base);
+                return j == t ? x + g1 : x;
+            });
     }
 }
 
