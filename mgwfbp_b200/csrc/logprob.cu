@@ -25,9 +25,10 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxTop = 32;
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnroll = 4;                 // 16-byte vectors that a thread keeps in flight
+constexpr int kUnroll = 4;                 // 16-byte vectors of a thread in a batch
+constexpr int kStages = 3;                 // batches of a warp on their way or in use
 constexpr int kBatch = 32 * kUnroll;       // vectors that a warp reads at a time
 constexpr int kMaxima = 128;               // maxima that a warp keeps; neighbouring batches share one beyond that
 constexpr int kCandidates = 512;
@@ -300,6 +301,40 @@ struct Row {
         has_head = part == 0;
         has_tail = part == splits - 1;
     }
+    // Calls use(i0, r) for each whole batch of this warp, vectors i0 + 32 k + lane.  The loads run kStages - 1 batches ahead,
+    // through a ring in shared memory of which every thread reads only what it has loaded itself.
+    template <typename F>
+    __device__ __forceinline__ void for_batches(uint4* ring, F use) const {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = v0 + warp * kBatch;
+        const int n = v1 - first < kBatch ? 0 : (v1 - first - kBatch) / (kWarps * kBatch) + 1;
+        const uint4* from = reinterpret_cast<const uint4*>(z + head) + first + lane;
+        uint4* mine = ring + warp * (kStages * kBatch) + lane;
+        const uint32_t slot = (uint32_t)__cvta_generic_to_shared(mine);
+        auto fetch = [&](int b) {
+            if (b < n) {
+#pragma unroll
+                for (int k = 0; k < kUnroll; ++k)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                 :: "r"(slot + ((b % kStages) * kBatch + k * 32) * 16), "l"(from + (long long)b * (kWarps * kBatch) + k * 32) : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int b = 0; b < kStages - 1; ++b) fetch(b);
+        for (int b = 0; b < n; ++b) {
+            fetch(b + kStages - 1);
+            asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
+            uint4 r[kUnroll];
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) r[k] = mine[(b % kStages) * kBatch + k * 32];
+            use(first + b * (kWarps * kBatch), r);
+        }
+    }
+    // first vector behind this warp's whole batches, for the few that are left (v1 where there are none)
+    __device__ __forceinline__ int rest() const {
+        const int first = v0 + (threadIdx.x >> 5) * kBatch;
+        return v1 - first < kBatch ? first : first + ((v1 - first - kBatch) / (kWarps * kBatch) + 1) * (kWarps * kBatch);
+    }
     __device__ __forceinline__ uint4 vec(int i) const { return reinterpret_cast<const uint4*>(z + head)[i]; }
     // the element at the edge that a thread of the block looks after (0 .. 15), or -1
     __device__ __forceinline__ int edge(int thread) const {
@@ -307,6 +342,8 @@ struct Row {
         return thread < 16 && has_tail && tail0 + thread - 8 < vocab ? tail0 + thread - 8 : -1;
     }
 };
+
+constexpr size_t kRingBytes = (size_t)kWarps * kStages * kBatch * 16;
 
 struct TopSpace {
     float maxima[kWarps][kMaxima];         // of the batches of a warp
@@ -320,7 +357,7 @@ struct TopSpace {
 // Sums of this block's part of the row; with TOP also the batches' maxima and the thread's own (most: minus infinity
 // where it has no vector).
 template <typename T, bool ENT, bool TOP>
-__device__ __forceinline__ Sums scan_row(const Row<T>& row, int shift, TopSpace* top, float& most) {
+__device__ __forceinline__ Sums scan_row(const Row<T>& row, uint4* ring, int shift, TopSpace* top, float& most) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Sums a;
     a.m = Fast<T>::start;
@@ -328,35 +365,33 @@ __device__ __forceinline__ Sums scan_row(const Row<T>& row, int shift, TopSpace*
     a.s = a.u = pair(0.f, 0.f);
     most = -INFINITY;
     int batch = 0;
-    for (int i0 = row.v0 + warp * kBatch; i0 < row.v1; i0 += kWarps * kBatch, ++batch) {
-        float m;
-        if (i0 + kBatch <= row.v1) {
-            uint4 r[kUnroll];
+    auto note = [&](float m) {                                       // the batch's maximum
+        most = max_nan(most, m);
+        const float w = warp_max_nan(m);
+        if (lane == 0) {
+            float* to = &top->maxima[warp][batch >> shift];
+            *to = (batch & ((1 << shift) - 1)) == 0 ? w : max_nan(*to, w);
+        }
+        ++batch;
+    };
+    row.for_batches(ring, [&](int, const uint4 (&r)[kUnroll]) {
+        const float m = Vec<T>::largest(r), up = max_nan(a.m, m);
+        if (up != a.m) raise_to<ENT>(a, up);
 #pragma unroll
-            for (int k = 0; k < kUnroll; ++k) r[k] = row.vec(i0 + k * 32 + lane);
-            m = Vec<T>::largest(r);
+        for (int k = 0; k < kUnroll; ++k) add_vector<T, ENT>(a, r[k]);
+        if (TOP) note(m);
+    });
+    const int i0 = row.rest();
+    if (i0 < row.v1) {                                               // less than a batch
+        float m = -INFINITY;
+        for (int i = i0 + lane; i < row.v1; i += 32) {
+            const uint4 r[1] = {row.vec(i)};
+            m = max_nan(m, Vec<T>::largest(r));
             const float up = max_nan(a.m, m);
             if (up != a.m) raise_to<ENT>(a, up);
-#pragma unroll
-            for (int k = 0; k < kUnroll; ++k) add_vector<T, ENT>(a, r[k]);
-        } else {                                                     // the last batch of the part
-            m = -INFINITY;
-            for (int i = i0 + lane; i < row.v1; i += 32) {
-                const uint4 r[1] = {row.vec(i)};
-                m = max_nan(m, Vec<T>::largest(r));
-                const float up = max_nan(a.m, m);
-                if (up != a.m) raise_to<ENT>(a, up);
-                add_vector<T, ENT>(a, r[0]);
-            }
+            add_vector<T, ENT>(a, r[0]);
         }
-        if (TOP) {
-            most = max_nan(most, m);
-            const float w = warp_max_nan(m);
-            if (lane == 0) {
-                float* to = &top->maxima[warp][batch >> shift];
-                *to = (batch & ((1 << shift) - 1)) == 0 ? w : max_nan(*to, w);
-            }
-        }
+        if (TOP) note(m);
     }
     const int j = row.edge(threadIdx.x);
     if (j >= 0) {
@@ -544,7 +579,7 @@ __device__ __forceinline__ int rank_of(Key x, const Key* keys, int n) {
 // The block's part of a row of a gradient.  pairs(Pair logits) and one(logit, column) give the values; the column `t` is
 // always done by one().  Whole vectors where logits and gradient start at the same place of a 16-byte block.
 template <typename T, bool READ, bool LIFT, typename FP, typename F1>
-__device__ __forceinline__ void write_row(const Row<T>& row, T* dz, long long t, FP pairs, F1 one) {
+__device__ __forceinline__ void write_row(const Row<T>& row, uint4* ring, T* dz, long long t, FP pairs, F1 one) {
     constexpr int N = Vec<T>::N;
     if (((unsigned long long)dz & 15) == ((unsigned long long)row.z & 15)) {
         uint4* to = reinterpret_cast<uint4*>(dz + row.head);
@@ -557,22 +592,15 @@ __device__ __forceinline__ void write_row(const Row<T>& row, T* dz, long long t,
             to[i] = Vec<T>::pack(f);
             if (i == ti) dz[t] = mgw_from_float<T>(one(READ ? mgw_to_float(row.z[t]) : 0.f, (int)t));
         };
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        for (int i0 = row.v0 + warp * kBatch; i0 < row.v1; i0 += kWarps * kBatch) {
-            if (i0 + kBatch <= row.v1) {
-                uint4 q[kUnroll];
+        const int lane = threadIdx.x & 31;
+        if (READ) {
+            row.for_batches(ring, [&](int i0, const uint4 (&r)[kUnroll]) {
 #pragma unroll
-                for (int k = 0; k < kUnroll; ++k)
-                    if (READ) q[k] = row.vec(i0 + k * 32 + lane);
-#pragma unroll
-                for (int k = 0; k < kUnroll; ++k) finish(q[k], i0 + k * 32 + lane);
-            } else {
-                for (int i = i0 + lane; i < row.v1; i += 32) {
-                    uint4 q;
-                    if (READ) q = row.vec(i);
-                    finish(q, i);
-                }
-            }
+                for (int k = 0; k < kUnroll; ++k) finish(r[k], i0 + k * 32 + lane);
+            });
+            for (int i = row.rest() + lane, end = min(row.v1, row.rest() + kBatch); i < end; i += 32) finish(row.vec(i), i);
+        } else {
+            for (int i = row.v0 + threadIdx.x; i < row.v1; i += kThreads) finish(make_uint4(0, 0, 0, 0), i);
         }
     } else {
         for (int j = row.head + row.v0 * N + threadIdx.x; j < row.head + row.v1 * N; j += kThreads)
@@ -584,7 +612,7 @@ __device__ __forceinline__ void write_row(const Row<T>& row, T* dz, long long t,
 
 template <typename T>
 __device__ __noinline__ void write_constant(const Row<T>& row, T* dz, float c) {
-    write_row<T, false, false>(row, dz, -1, [=](Pair) { return pair(c, c); }, [=](float, int) { return c; });
+    write_row<T, false, false>(row, nullptr, dz, -1, [=](Pair) { return pair(c, c); }, [=](float, int) { return c; });
 }
 
 // A row whose maximum is at the edge of the range: -p (base + slope log2 p) + g1 delta, one by one.
@@ -600,14 +628,14 @@ __device__ __noinline__ void write_careful(const Row<T>& row, T* dz, float m, fl
 
 // g (p - delta), the gradient of one row's loss: 2^(L z - M) times g / s
 template <typename T>
-__device__ __forceinline__ void write_loss_gradient(const Row<T>& row, T* dz, float m, float log2_s, float g, long long t) {
+__device__ __forceinline__ void write_loss_gradient(const Row<T>& row, uint4* ring, T* dz, float m, float log2_s, float g, long long t) {
     if (careful<T>(m)) {
         write_careful(row, dz, m, log2_s, -g, 0.f, -g, t);
         return;
     }
     const float M = __fmul_rn(m, kLog2e), gs = g * exp2f(-log2_s);
     write_row<T, true, false>(
-        row, dz, t, [=](Pair v) { return mul2(exp2_fast(fma2(v, pair(kLog2e, kLog2e), pair(-M, -M))), pair(gs, gs)); },
+        row, ring, dz, t, [=](Pair v) { return mul2(exp2_fast(fma2(v, pair(kLog2e, kLog2e), pair(-M, -M))), pair(gs, gs)); },
         [=](float v, int j) {
             const float x = exp2_fast(fmaf(v, kLog2e, -M)) * gs;
             return j == t ? x - g : x;
@@ -616,9 +644,10 @@ __device__ __forceinline__ void write_loss_gradient(const Row<T>& row, T* dz, fl
 
 // ------------------------------------------------------------------------------------------------------------ forward
 template <typename T, bool ENT, bool TOP, bool LOSS>
-__global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
     extern __shared__ __align__(16) unsigned char dynamic[];
-    TopSpace* top = reinterpret_cast<TopSpace*>(dynamic);            // only with TOP
+    uint4* ring = reinterpret_cast<uint4*>(dynamic);
+    TopSpace* top = reinterpret_cast<TopSpace*>(dynamic + kRingBytes);       // only with TOP
     __shared__ Stats parts[kWarps];
     __shared__ Stats of_block;
     __shared__ Key block_list[kMaxTop];
@@ -645,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(RowArgs a) {
         if (TOP)
             while (((row.v1 - row.v0) / (kWarps * kBatch) >> shift) >= kMaxima) ++shift;
         float most;
-        Stats x = block_join<ENT>(scan_row<T, ENT, TOP>(row, shift, top, most), parts);
+        Stats x = block_join<ENT>(scan_row<T, ENT, TOP>(row, ring, shift, top, most), parts);
         if (a.splits > 1) {
             cg::cluster_group cluster = cg::this_cluster();
             if (threadIdx.x == 0) of_block = x;
@@ -692,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(RowArgs a) {
         }
         if (LOSS && a.dz != nullptr) {                               // the row was just read: it comes from L2
             T* dz = static_cast<T*>(a.dz) + r * a.dz_ld;
-            if (fine && valid) write_loss_gradient(row, dz, x.m, log2_s, a.expected / (float)*a.count, t);
+            if (fine && valid) write_loss_gradient(row, ring, dz, x.m, log2_s, a.expected / (float)*a.count, t);
             else write_constant(row, dz, mgw_nan());
         }
         if (a.splits > 1) cg::this_cluster().sync();                 // until here the others may read this block's memory
@@ -762,7 +791,9 @@ struct GradArgs {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(GradArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) logprob_bwd_kernel(GradArgs a) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    uint4* ring = reinterpret_cast<uint4*>(dynamic);
     const float g_loss = a.g_loss != nullptr ? *a.g_loss : 0.f;
     if (a.written && g_loss == a.expected) return;
     for (long long task = blockIdx.x; task < a.rows * a.splits; task += gridDim.x) {
@@ -781,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(GradArgs a) {
             continue;
         }
         if (a.g_loss != nullptr) {
-            write_loss_gradient(row, dz, m, log2_s, g_loss / (float)*a.count, t);
+            write_loss_gradient(row, ring, dz, m, log2_s, g_loss / (float)*a.count, t);
             continue;
         }
         // g1 (delta - p) - g2 p (ln p + H); with d = L z - M:  p = 2^d / s,  ln p = ln 2 (d - log2 s)
@@ -793,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(GradArgs a) {
         }
         const float base = g1 + g2 * h - slope * log2_s, rs = -exp2f(-log2_s);
         write_row<T, true, true>(
-            row, dz, t,
+            row, ring, dz, t,
             [=](Pair v) {
                 const Pair d = fma2(v, pair(kLog2e, kLog2e), pair(-M, -M));
                 return mul2(mul2(exp2_fast(d), pair(rs, rs)), fma2(pair(slope, slope), d, pair(base, base)));
@@ -814,7 +845,7 @@ bool bad_rows(const void* z, long long ld, long long rows, int vocab, int dtype,
 
 template <typename T, bool ENT, bool TOP, bool LOSS>
 int launch_fwd(const RowArgs& a, cudaStream_t stream) {
-    const size_t smem = TOP ? sizeof(TopSpace) : 0;
+    const size_t smem = kRingBytes + (TOP ? sizeof(TopSpace) : 0);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * a.splits));
     cfg.blockDim = dim3(kThreads);
@@ -835,12 +866,12 @@ int launch_fwd(const RowArgs& a, cudaStream_t stream) {
     return a.top > 0 ? launch_fwd<T, true, true, false>(a, stream) : launch_fwd<T, true, false, false>(a, stream);
 }
 
-// Blocks per row: one as long as the rows alone give two blocks to every SM, else up to 8 (a portable cluster) that have
+// Blocks per row: one as long as the rows alone give four blocks to every SM, else up to 8 (a portable cluster) that have
 // at least 128 vectors each.
 int splits_of(long long rows, int vocab, int dtype) {
     const int per = dtype == MGW_F32 ? 4 : 8;
     int splits = 1;
-    while (splits < 8 && rows * splits < 148 * 2 && vocab / per / (splits * 2) >= 128) splits *= 2;
+    while (splits < 8 && rows * splits < 148 * 4 && vocab / per / (splits * 2) >= 128) splits *= 2;
     return splits;
 }
 
@@ -879,9 +910,9 @@ extern "C" int mgw_logprob_bwd(const void* z, long long ld, long long rows, int 
     cudaStream_t s = (cudaStream_t)stream;
     const long long tasks = rows * a.splits;
     const unsigned grid = (unsigned)(tasks < 148 * 8 ? tasks : 148 * 8);
-    if (dtype == MGW_F32) logprob_bwd_kernel<float><<<grid, kThreads, 0, s>>>(a);
-    else if (dtype == MGW_F16) logprob_bwd_kernel<__half><<<grid, kThreads, 0, s>>>(a);
-    else logprob_bwd_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
+    if (dtype == MGW_F32) logprob_bwd_kernel<float><<<grid, kThreads, kRingBytes, s>>>(a);
+    else if (dtype == MGW_F16) logprob_bwd_kernel<__half><<<grid, kThreads, kRingBytes, s>>>(a);
+    else logprob_bwd_kernel<__nv_bfloat16><<<grid, kThreads, kRingBytes, s>>>(a);
     MGW_CUDA_CHECK(cudaGetLastError());
     return MGW_OK;
 }
