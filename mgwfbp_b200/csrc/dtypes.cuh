@@ -51,6 +51,11 @@ __device__ __forceinline__ typename MgwRaw<N * sizeof(T)>::type mgw_pack(const f
     return u.raw;
 }
 
+// Programmatic dependent launch: a kernel may be launched while the one before it still runs, and waits here for that
+// one's end and results.  Without the launch attribute both do nothing.
+__device__ __forceinline__ void mgw_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void mgw_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ float mgw_nan() { return __int_as_float(0x7fc00000); }
 
 // The token with index i of an int32 (wide = 0) or int64 (wide = 1) list.

@@ -16,11 +16,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-// The kernels of the gradient follow each other closely: each is launched while the one before still runs (programmatic
-// dependent launch) and waits for its results here.  Without the launch attribute both are no-ops.
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
+// The kernels of the gradient follow each other closely: each is launched while the one before still runs.
 template <typename... P, typename... A>
 int launch_dependent(void (*kernel)(P...), long long grid, int threads, size_t smem, cudaStream_t stream, A... args) {
     cudaLaunchConfig_t cfg = {};
@@ -112,8 +108,8 @@ __device__ __forceinline__ uint2 sort_entry(const SortPass& p, long long i, bool
 __global__ void __launch_bounds__(kSortThreads) sort_hist_kernel(SortPass p) {
     extern __shared__ uint32_t hist[];
     const int bins = 1 << p.bits;
-    let_next_start();
-    wait_for_previous();
+    mgw_let_next_start();
+    mgw_wait_for_previous();
     for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
     __syncthreads();
     const long long i0 = (long long)blockIdx.x * kSortTile;
@@ -129,8 +125,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_hist_kernel(SortPass p) {
 // One warp per digit: exclusive scan over the tiles, total of the digit.
 __global__ void __launch_bounds__(256) sort_scan_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ totals, int bins, int tiles) {
     const int bin = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    let_next_start();
-    wait_for_previous();
+    mgw_let_next_start();
+    mgw_wait_for_previous();
     if (bin >= bins) return;
     uint32_t* row = counts + (long long)bin * tiles;
     uint32_t before = 0;
@@ -156,8 +152,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) 
     uint16_t* cnt = reinterpret_cast<uint16_t*>(smem + bins);         // [warps][bins] entries of the warps
     __shared__ uint32_t warp_sum[kWarps];
     for (int b = threadIdx.x; b < bins * kWarps; b += kSortThreads) cnt[b] = 0;
-    let_next_start();
-    wait_for_previous();
+    mgw_let_next_start();
+    mgw_wait_for_previous();
     // exclusive scan of the digits' totals: a thread owns bins / 512 neighbouring digits
     const int per = (bins + kSortThreads - 1) / kSortThreads;
     uint32_t mine = 0;
@@ -255,7 +251,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThrea
     extern __shared__ __align__(16) unsigned char dynamic[];
     ClusterSmem& m = *reinterpret_cast<ClusterSmem*>(dynamic);
     cg::cluster_group cluster = cg::this_cluster();
-    let_next_start();
+    mgw_let_next_start();
     if (blockIdx.x >= kCluster) {
         fill_zero(zeros, zero_bytes, blockIdx.x - kCluster, gridDim.x - kCluster);
         return;
@@ -428,8 +424,8 @@ __device__ __forceinline__ void zero_rows(const GradArgs& a, long long block) {
 
 template <typename T, int VEC, int NV>
 __global__ void __launch_bounds__(256) grad_chunks_kernel(GradArgs a) {
-    let_next_start();
-    wait_for_previous();
+    mgw_let_next_start();
+    mgw_wait_for_previous();
     if ((int)blockIdx.x < a.zero_blocks) {
         zero_rows<T, VEC>(a, blockIdx.x);
         return;
@@ -501,7 +497,7 @@ __global__ void __launch_bounds__(256) grad_chunks_kernel(GradArgs a) {
 // Runs that cross borders of chunks: the warp of the chunk in which a run starts adds up the partial sums.
 template <typename T, int VEC, int NV>
 __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a) {
-    wait_for_previous();
+    mgw_wait_for_previous();
     const int lane = threadIdx.x & 31;
     const long long task = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (task >= (long long)(a.chunks - 1) * a.slabs) return;

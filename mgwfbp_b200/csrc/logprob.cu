@@ -308,26 +308,30 @@ struct Row {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = v0 + warp * kBatch;
         const int n = v1 - first < kBatch ? 0 : (v1 - first - kBatch) / (kWarps * kBatch) + 1;
         const uint4* from = reinterpret_cast<const uint4*>(z + head) + first + lane;
-        uint4* mine = ring + warp * (kStages * kBatch) + lane;
-        const uint32_t slot = (uint32_t)__cvta_generic_to_shared(mine);
-        auto fetch = [&](int b) {
-            if (b < n) {
+        const uint4* end = from + (long long)n * (kWarps * kBatch);
+        const uint4* mine = ring + warp * (kStages * kBatch) + lane;
+        const uint32_t base = (uint32_t)__cvta_generic_to_shared(mine);
+        uint32_t put = 0, get = 0;                                   // slots, in bytes from the thread's first
+        auto fetch = [&]() {
+            if (from < end) {
 #pragma unroll
                 for (int k = 0; k < kUnroll; ++k)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                                 :: "r"(slot + ((b % kStages) * kBatch + k * 32) * 16), "l"(from + (long long)b * (kWarps * kBatch) + k * 32) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(base + put + k * 512), "l"(from + k * 32) : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
+            from += kWarps * kBatch;
+            put = put == (kStages - 1) * kBatch * 16 ? 0 : put + kBatch * 16;
         };
 #pragma unroll
-        for (int b = 0; b < kStages - 1; ++b) fetch(b);
-        for (int b = 0; b < n; ++b) {
-            fetch(b + kStages - 1);
+        for (int b = 0; b < kStages - 1; ++b) fetch();
+        for (int i0 = first, i1 = first + n * (kWarps * kBatch); i0 < i1; i0 += kWarps * kBatch) {
+            fetch();
             asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
             uint4 r[kUnroll];
 #pragma unroll
-            for (int k = 0; k < kUnroll; ++k) r[k] = mine[(b % kStages) * kBatch + k * 32];
-            use(first + b * (kWarps * kBatch), r);
+            for (int k = 0; k < kUnroll; ++k) r[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(mine) + get + k * 512);
+            get = get == (kStages - 1) * kBatch * 16 ? 0 : get + kBatch * 16;
+            use(i0, r);
         }
     }
     // first vector behind this warp's whole batches, for the few that are left (v1 where there are none)
@@ -589,7 +593,7 @@ __device__ __forceinline__ void write_row(const Row<T>& row, uint4* ring, T* dz,
             if (READ) Vec<T>::template values<LIFT>(q, f);
 #pragma unroll
             for (int k = 0; k < N / 2; ++k) f[k] = pairs(f[k]);
-            to[i] = Vec<T>::pack(f);
+            __stcs(&to[i], Vec<T>::pack(f));                         // not read again here
             if (i == ti) dz[t] = mgw_from_float<T>(one(READ ? mgw_to_float(row.z[t]) : 0.f, (int)t));
         };
         const int lane = threadIdx.x & 31;
@@ -719,6 +723,7 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
                     a.top_logprob[r * a.top + k] = fine ? ln_prob<T>(mgw_to_float(row.z[j]), x.m, log2_s) : mgw_nan();
                 }
         }
+        if (LOSS) mgw_wait_for_previous();                               // the count of rows
         if (LOSS && a.dz != nullptr) {                               // the row was just read: it comes from L2
             T* dz = static_cast<T*>(a.dz) + r * a.dz_ld;
             if (fine && valid) write_loss_gradient(row, ring, dz, x.m, log2_s, a.expected / (float)*a.count, t);
@@ -726,6 +731,7 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
         }
         if (a.splits > 1) cg::this_cluster().sync();                 // until here the others may read this block's memory
     }
+    if (LOSS) mgw_wait_for_previous();                                   // the counter, also for rows that are padding
     if (LOSS && a.loss != nullptr && part == 0) {
         // the block that finishes last adds up the rows: thread i rows i, i + 256, ..., the same order every time
         __shared__ bool last;
@@ -755,6 +761,7 @@ __global__ void __launch_bounds__(1024) count_rows_kernel(const void* __restrict
                                                           int mean, int* __restrict__ count, unsigned int* __restrict__ done,
                                                           float* __restrict__ loss) {
     __shared__ int kept[32];
+    mgw_let_next_start();
     int k = 0;
     if (mean)
         for (long long i = threadIdx.x; i < rows; i += 1024) k += mgw_token(tokens, wide, i) != ignore;
@@ -851,11 +858,20 @@ int launch_fwd(const RowArgs& a, cudaStream_t stream) {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (a.splits > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = a.splits; attr[n].val.clusterDim.y = 1; attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (LOSS) {                                                      // reads the rows while the launch before counts them
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = a.splits > 1 ? 1 : 0;
+    cfg.numAttrs = n;
     MGW_CUDA_CHECK(cudaLaunchKernelEx(&cfg, logprob_fwd_kernel<T, ENT, TOP, LOSS>, a));
     return MGW_OK;
 }
@@ -866,17 +882,23 @@ int launch_fwd(const RowArgs& a, cudaStream_t stream) {
     return a.top > 0 ? launch_fwd<T, true, true, false>(a, stream) : launch_fwd<T, true, false, false>(a, stream);
 }
 
+constexpr long long kResident = 148 * 8;                               // blocks that run at once
+constexpr long long kInL2 = 40LL << 20;                               // bytes of rows that are still in L2 when they are read again
+
 // Blocks per row: one as long as the rows alone give four blocks to every SM, else up to 8 (a portable cluster) that have
-// at least 128 vectors each.
-int splits_of(long long rows, int vocab, int dtype) {
+// at least 128 vectors each.  Where rows are read twice (`twice`, the loss and its gradient), as many that the rows in
+// flight stay in L2.
+int splits_of(long long rows, int vocab, int dtype, bool twice) {
     const int per = dtype == MGW_F32 ? 4 : 8;
     int splits = 1;
-    while (splits < 8 && rows * splits < 148 * 4 && vocab / per / (splits * 2) >= 128) splits *= 2;
+    while (splits < 8 && vocab / per / (splits * 2) >= 128 &&
+           (rows * splits < kResident / 2 || (twice && (rows < kResident / splits ? rows : kResident / splits) * vocab * (16 / per) > kInL2)))
+        splits *= 2;
     return splits;
 }
 
 int launch_fwd(RowArgs& a, int dtype, cudaStream_t stream) {
-    a.splits = splits_of(a.rows, a.vocab, dtype);
+    a.splits = splits_of(a.rows, a.vocab, dtype, a.dz != nullptr);
     return dtype == MGW_F32 ? launch_fwd<float>(a, stream) : dtype == MGW_F16 ? launch_fwd<__half>(a, stream) : launch_fwd<__nv_bfloat16>(a, stream);
 }
 
@@ -906,7 +928,7 @@ extern "C" int mgw_logprob_bwd(const void* z, long long ld, long long rows, int 
         (g_loss != nullptr && count == nullptr) || (written && g_loss == nullptr))
         return MGW_ERR_ARG;
     GradArgs a = {z, ld, rows, vocab, tokens, wide, ignore, reinterpret_cast<const float2*>(stats), g_entropy ? entropy : nullptr,
-                  g_logprob, g_entropy, g_loss, count, written, expected, dz, dz_ld, splits_of(rows, vocab, dtype)};
+                  g_logprob, g_entropy, g_loss, count, written, expected, dz, dz_ld, splits_of(rows, vocab, dtype, false)};
     cudaStream_t s = (cudaStream_t)stream;
     const long long tasks = rows * a.splits;
     const unsigned grid = (unsigned)(tasks < 148 * 8 ? tasks : 148 * 8);
