@@ -251,13 +251,15 @@ class TrainStep:
     def check_status(self) -> None:
         """Raise :class:`CommTimeoutError` when a communication kernel of an earlier step gave up waiting for a peer
         (the kernels record that in host-mapped memory; reading it costs no synchronisation, so this runs every step,
-        graph replay included), or when the weight-gradient GEMM reported a failed wait."""
+        graph replay included), when the weight-gradient GEMM reported a failed wait, or when a kernel met a token
+        outside the vocabulary (:class:`~mgwfbp_b200.ops._tokens.TokenIndexError`)."""
         comm = getattr(self.optimizer, '_comm', None)
         check = getattr(comm, 'check_status', None)
         if check is not None:
             check()
-        from .ops import wgrad
+        from .ops import _tokens, wgrad
         wgrad.check_status_nosync()
+        _tokens.check_status_nosync()
 
     def _collect(self, force: int) -> None:
         if self.cuda:

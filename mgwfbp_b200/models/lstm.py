@@ -5,7 +5,8 @@
 Linear(1500, V)`` with the parameter names of reference ``models/lstm.py:5-47``
 (``word_embeddings.weight``, ``lstm.weight_ih_l0`` ..., ``sm_fc.weight``).  The recurrent part is
 either ``torch.nn.LSTM`` (cuDNN) or this package's :class:`~mgwfbp_b200.ops.lstm.FusedLSTM`,
-which exposes the same parameter names and shapes.
+the embedding either ``torch.nn.Embedding`` or :class:`~mgwfbp_b200.ops.embedding.FusedEmbedding`;
+both expose the same parameter names and shapes.
 """
 from __future__ import annotations
 
@@ -15,7 +16,7 @@ import torch.nn as nn
 
 class lstm(nn.Module):
     def __init__(self, vocab_size, embedding_dim=1500, num_steps=35, batch_size=20, num_layers=2,
-                 dp_keep_prob=0.35, fused=False):
+                 dp_keep_prob=0.35, fused=False, fused_embedding=False):
         super().__init__()
         self.name = 'lstm'
         self.embedding_dim = embedding_dim
@@ -25,7 +26,11 @@ class lstm(nn.Module):
         self.dp_keep_prob = dp_keep_prob
         self.num_layers = num_layers
         self.dropout = nn.Dropout(1 - dp_keep_prob)
-        self.word_embeddings = nn.Embedding(vocab_size, embedding_dim)
+        if fused_embedding:
+            from ..ops.embedding import FusedEmbedding
+            self.word_embeddings = FusedEmbedding(vocab_size, embedding_dim)
+        else:
+            self.word_embeddings = nn.Embedding(vocab_size, embedding_dim)
         if fused:
             from ..ops.lstm import FusedLSTM
             self.lstm = FusedLSTM(embedding_dim, embedding_dim, num_layers=num_layers, dropout=1 - dp_keep_prob)

@@ -28,7 +28,7 @@ import numpy as np
 import torch
 
 from ... import settings
-from ...ops import _lib, counters
+from ...ops import _lib, clip, counters
 from ...ops.tables import GroupTable, HyperTable, ensure_momentum_buffers, param_group_index
 from ...settings import logger
 from .. import runtime
@@ -465,7 +465,12 @@ class NvlComm(Communicator):
                 counters.bump('multi_tensor_sgd')
                 return loss
         if opt._norm_clip is not None:
-            torch.nn.utils.clip_grad_norm_([p for p in opt._requires_update], opt._norm_clip)
+            # in the order of the parameter groups: the same on every rank, so that all get the same norm bit for bit
+            params = [p for g in opt.param_groups for p in g['params'] if p in opt._requires_update and p.grad is not None]
+            if clip.supported([p.grad for p in params]):
+                clip.clip_grad_norm_(params, opt._norm_clip)
+            else:
+                torch.nn.utils.clip_grad_norm_(params, opt._norm_clip)
         opt._base_cls.step(opt)
         return loss
 

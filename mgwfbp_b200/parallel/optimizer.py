@@ -437,11 +437,17 @@ class _DistributedMixin:
         if self._norm_clip is not None and not self.local and getattr(self, '_fast_sgd', None) is None:
             # global L2-norm clip of the averaged gradient (the reference's loop calls
             # clip_grad_norm_ between synchronize() and step(), dist_trainer.py:89-94)
-            self._unscale_grads_()
+            from ..ops import clip
+            params = [p for g in self.param_groups for p in g['params'] if p.grad is not None]
+            fused = clip.supported([p.grad for p in params])         # one GPU's dense fp32 / fp16 / bf16 gradients
+            if fused:
+                clip.clip_grad_norm_(params, self._norm_clip, grad_scale=self._grad_scale)
+            else:
+                self._unscale_grads_()
             scale, self._grad_scale = self._grad_scale, 1.0          # already divided out
             try:
-                params = [p for g in self.param_groups for p in g['params'] if p.grad is not None]
-                torch.nn.utils.clip_grad_norm_(params, self._norm_clip)
+                if not fused:
+                    torch.nn.utils.clip_grad_norm_(params, self._norm_clip)
                 return self._local_step(closure)
             finally:
                 self._grad_scale = scale

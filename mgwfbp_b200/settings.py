@@ -72,6 +72,10 @@ FUSE_MODULES = _env_flag('FUSE', True)
 # library's LSTM) is used.  Measured on B200 (batch 20, 35 steps, 1500 hidden, whole training step): 2.60 ms with the
 # kernels here, 2.56 ms with the library's -- the named kernels are on the hot path at a cost of 1.6 %.
 FUSE_LSTM = _env_flag('FUSE_LSTM', True)
+# The two ends of the PTB model, when it is built with fused modules on a GPU: word_embeddings is
+# mgwfbp_b200.ops.embedding.FusedEmbedding (gradient by sorted tokens) and the criterion is
+# mgwfbp_b200.ops.logprob.FusedCrossEntropyLoss (gradient of the logits written while a row is in L2).
+FUSE_LM_OPS = _env_flag('FUSE_LM_OPS', True)
 # How many algorithms cuDNN's benchmark mode may time per convolution shape (-1: leave PyTorch's default of 10, 0: all).
 CUDNN_BENCHMARK_LIMIT = int(_env_str('CUDNN_BENCHMARK_LIMIT', '-1'))
 # Keep convolutional models and their inputs in channels-last (NHWC) memory format on the GPU.

@@ -67,6 +67,7 @@ class DLTrainer:
         self.loss_scale = float(settings.LOSS_SCALE) if self.fp16 else 1.0
         self.fuse = (self.is_cuda and settings.FUSE_MODULES) if fuse is None else bool(fuse)
         self.channels_last = (self.is_cuda and settings.CHANNELS_LAST) if channels_last is None else bool(channels_last)
+        self.fuse_lm_ops = self.fuse and settings.FUSE_LM_OPS
         if seed is not None:
             torch.manual_seed(seed)
         self.train_sampler = None
@@ -85,7 +86,7 @@ class DLTrainer:
             kwargs = {}
             if dnn == 'lstm':
                 kwargs = dict(vocab_size=self.vocab_size, batch_size=self.batch_size, num_steps=self.num_steps,
-                              fused_lstm=self.fuse and settings.FUSE_LSTM)
+                              fused_lstm=self.fuse and settings.FUSE_LSTM, fused_embedding=self.fuse_lm_ops)
             elif dnn == 'lstman4':
                 kwargs = dict(datapath=None if _is_synthetic(data_dir) else data_dir)
             is_conv = dnn not in ('lstm', 'lstman4', 'fcn5net', 'lr')
@@ -108,7 +109,10 @@ class DLTrainer:
         self.master = master
         if dist:
             runtime.init()
-        if self.dataset != 'an4':
+        if self.dataset == 'ptb' and self.fuse_lm_ops:
+            from .ops.logprob import FusedCrossEntropyLoss
+            self.criterion = FusedCrossEntropyLoss(expected_grad=self.loss_scale)
+        elif self.dataset != 'an4':
             self.criterion = nn.CrossEntropyLoss().to(self.device)
         else:
             self.criterion = nn.CTCLoss(blank=0, reduction='sum', zero_infinity=True)
@@ -143,6 +147,7 @@ class DLTrainer:
         self.train_acc_top1: List[Any] = []
         self._acc_sum_t, self._acc_steps = None, 0
         self.num_of_updates_during_comm = 0
+        self.word_stats = None                            # next-word statistics of the last test() of the PTB model
         self._loss_t: Optional[torch.Tensor] = None       # loss of the last train() call, on device
         self._epoch_loss_t: Optional[torch.Tensor] = None
         logger.info('num_batches_per_epoch: %d' % self.num_batches_per_epoch)
@@ -584,6 +589,9 @@ class DLTrainer:
             if self.dnn not in ('lstm', 'lstman4'):
                 self.train_acc_top1.append(self.cal_accuracy(outputs.detach(), labels, topk=(1,))[0])
             self.train_iter += 1
+        if self.fuse_lm_ops:
+            from .ops._tokens import check_status_nosync
+            check_status_nosync()                     # a word outside the vocabulary, met by a launch that has finished
         self.num_of_updates_during_comm += 1
         self._loss_t = loss_acc / num_of_iters if loss_acc is not None else None
         self.timer += time.time() - s
@@ -600,8 +608,10 @@ class DLTrainer:
     # ------------------------------------------------------------------ evaluation
     def test(self, epoch):
         self.net.eval()
+        from .ops._tokens import check_status_nosync
+        from .ops.logprob import token_log_probs
         test_loss, costs, total_steps, total_iters, total, total_wer = 0.0, 0.0, 0, 0, 0, 0.0
-        top1, top5 = [], []
+        top1, top5, entropy = [], [], []
         with torch.no_grad():
             for data in self.testloader:
                 if self.dnn == 'lstman4':
@@ -620,6 +630,12 @@ class DLTrainer:
                     if self.dnn == 'lstm':
                         costs += float(loss) * self.net.num_steps
                         total_steps += self.net.num_steps
+                        words = token_log_probs(outputs, labels, top=min(5, outputs.size(-1)))
+                        hit = words.top_tokens == labels.unsqueeze(-1)
+                        top1.append(100.0 * float(hit[..., 0].float().mean()))
+                        top5.append(100.0 * float(hit.any(-1).float().mean()))
+                        entropy.append(float(words.entropy.mean()))
+                        check_status_nosync()
                     else:
                         a1, a5 = self.cal_accuracy(outputs, labels, topk=(1, 5))
                         top1.append(float(a1))
@@ -634,6 +650,11 @@ class DLTrainer:
         else:
             acc, acc5 = float(np.mean(top1)), float(np.mean(top5))
         logger.info('Epoch %d, lr: %f, val loss: %f, val top-1 acc: %f, top-5 acc: %f' % (epoch, self.lr, test_loss, acc, acc5))
+        if self.dnn == 'lstm' and top1:
+            # the line above carries the perplexity where other models have their accuracy, as the reference's does
+            self.word_stats = {'top1': float(np.mean(top1)), 'top5': float(np.mean(top5)), 'entropy': float(np.mean(entropy))}
+            logger.info('Epoch %d, next word: top-1 acc: %f, top-5 acc: %f, mean entropy: %f' % (
+                epoch, self.word_stats['top1'], self.word_stats['top5'], self.word_stats['entropy']))
         self.net.train()
         return acc
 
