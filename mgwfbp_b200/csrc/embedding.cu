@@ -38,42 +38,161 @@ constexpr int kSortItems = 4;
 constexpr int kSortTile = kSortThreads * kSortItems;
 constexpr int kMaxDigitBits = 10;
 
-// ------------------------------------------------------------------------------------------------------------ lookup
-constexpr int lookup_unroll(int bytes) { return bytes >= 16 ? 4 : bytes == 4 ? 8 : 16; }
+// --------------------------------------------------------------------------------------------------- blocks of a row
+// Rows move in blocks of 16 bytes.  EXACT: all rows of both matrices begin on 16-byte boundaries and consist of whole
+// blocks.  Otherwise every row is aligned differently: a block is cut out of two aligned vectors when it is read, and put
+// together from two lanes' values when it is stored.
+template <typename T> constexpr int per_block() { return 16 / (int)sizeof(T); }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256)
+// Elements between the last 16-byte boundary and the row.
+template <typename T>
+__device__ __forceinline__ int lead_of(const T* row) { return (int)(((unsigned long long)row & 15) / sizeof(T)); }
+
+struct Cut { uint4 x, y; int at; };        // 16 bytes from byte `at` of the 32 in x, y
+
+// Whether the vectors around every block of a row lie in the matrix [lo, hi), also those that its edges are cut out of.
+template <typename T>
+__device__ __forceinline__ bool inside(const T* row, int dim, const char* lo, const char* hi) {
+    return reinterpret_cast<const char*>(row) - 31 >= lo && reinterpret_cast<const char*>(row + dim) + 32 <= hi;
+}
+
+// The columns [c0, c0 + N); c0 may be up to N - 1 below the row's first column, or in its last block.
+template <typename T, bool EXACT>
+__device__ __forceinline__ Cut load_block(const T* row, int c0) {
+    const char* s = reinterpret_cast<const char*>(row + c0);
+    Cut r;
+    r.at = EXACT ? 0 : (int)((unsigned long long)s & 15);
+    r.x = *reinterpret_cast<const uint4*>(s - r.at);
+    if (!EXACT) r.y = *reinterpret_cast<const uint4*>(s - r.at + 16);
+    return r;
+}
+
+// The same for a row at the ends of the matrix: element by element, zero outside [0, dim).
+template <typename T>
+__device__ __noinline__ uint4 gather_block(const T* row, int c0, int dim) {
+    MgwVec<T, per_block<T>()> v;
+    v.raw = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < per_block<T>(); ++e)
+        if (c0 + e >= 0 && c0 + e < dim) v.v[e] = row[c0 + e];
+    return v.raw;
+}
+
+// The block that a Cut holds.  (Selects instead of a branch for each offset: these kernels are large enough that a copy
+// of their inner loop for each offset costs more in instruction fetches than it saves.)
+template <bool EXACT>
+__device__ __forceinline__ uint4 take(const Cut& c) {
+    if (EXACT) return c.x;
+    const uint32_t bits = (c.at & 3) * 8;
+    const bool two = c.at & 8, one = c.at & 4;
+    const uint32_t a0 = two ? c.x.z : c.x.x, a1 = two ? c.x.w : c.x.y, a2 = two ? c.y.x : c.x.z, a3 = two ? c.y.y : c.x.w,
+                   a4 = two ? c.y.z : c.y.x, a5 = two ? c.y.w : c.y.y;
+    const uint32_t b0 = one ? a1 : a0, b1 = one ? a2 : a1, b2 = one ? a3 : a2, b3 = one ? a4 : a3, b4 = one ? a5 : a4;
+    return make_uint4(__funnelshift_r(b0, b1, bits), __funnelshift_r(b1, b2, bits), __funnelshift_r(b2, b3, bits),
+                      __funnelshift_r(b3, b4, bits));
+}
+
+// The elements of a block whose bits are set, one by one: the ends of a row.  Kept small, it is executed rarely.
+__device__ __forceinline__ void store_element(float* to, const uint4& v, int e) {
+    *to = __uint_as_float(e & 2 ? (e & 1 ? v.w : v.z) : (e & 1 ? v.y : v.x));
+}
+template <typename T>
+__device__ __forceinline__ void store_element(T* to, const uint4& v, int e) {
+    const uint32_t w = e & 4 ? (e & 2 ? v.w : v.z) : (e & 2 ? v.y : v.x);
+    *reinterpret_cast<uint16_t*>(to) = (uint16_t)(e & 1 ? w >> 16 : w);
+}
+template <typename T>
+__device__ __forceinline__ void store_some(T* at, const uint4& v, unsigned which) {
+#pragma unroll 1
+    for (; which != 0; which &= which - 1) {
+        const int e = __ffs(which) - 1;
+        store_element(at + e, v, e);
+    }
+}
+// Bits of the elements [from, to) of a block.
+__device__ __forceinline__ unsigned range_bits(int from, int to) {
+    return from >= to ? 0u : ((1u << to) - 1u) & ~((1u << max(from, 0)) - 1u);
+}
+
+// A block that begins on a boundary, or the part of it in [0, dim).
+template <typename T, bool EXACT>
+__device__ __forceinline__ void store_block(T* row, int c0, int dim, const uint4& v) {
+    if (EXACT || (c0 >= 0 && c0 + per_block<T>() <= dim)) {
+        __stcs(reinterpret_cast<uint4*>(row + c0), v);
+        return;
+    }
+    store_some(row + c0, v, range_bits(-c0, min(per_block<T>(), dim - c0)));
+}
+
+// A warp's 32 neighbouring blocks, lane's at column c0 (all lanes take part; those with c0 >= dim have nothing).  With the
+// row `lead` elements behind a boundary, a lane puts the last `lead` elements of the lane before it in front of its own; what
+// no vector covers at the ends goes element by element.
+template <typename T, bool EXACT>
+__device__ __forceinline__ void store_blocks(T* row, int c0, int dim, const uint4& v) {
+    constexpr int N = per_block<T>();
+    if (EXACT) {
+        if (c0 < dim) __stcs(reinterpret_cast<uint4*>(row + c0), v);
+        return;
+    }
+    const int lane = threadIdx.x & 31, lead = lead_of(row);
+    Cut c;
+    c.x.x = __shfl_up_sync(0xffffffffu, v.x, 1);
+    c.x.y = __shfl_up_sync(0xffffffffu, v.y, 1);
+    c.x.z = __shfl_up_sync(0xffffffffu, v.z, 1);
+    c.x.w = __shfl_up_sync(0xffffffffu, v.w, 1);
+    c.y = v;
+    c.at = 16 - lead * (int)sizeof(T);
+    const bool whole = c0 + N - lead <= dim && (lane > 0 || lead == 0);
+    const bool next = __shfl_down_sync(0xffffffffu, (int)whole, 1) && lane < 31;
+    if (whole) __stcs(reinterpret_cast<uint4*>(row + c0 - lead), lead == 0 ? v : take<false>(c));
+    const int begin = whole ? N - lead : 0, stop = min(next ? N - lead : N, dim - c0);
+    if (begin < stop) store_some(row + c0, v, range_bits(begin, stop));
+}
+
+// ------------------------------------------------------------------------------------------------------------ lookup
+// Blocks that a lane keeps in flight; one more for rows between boundaries, which may have a block more than their length.
+constexpr int lookup_unroll(bool exact) { return exact ? 4 : 5; }
+
+template <typename T, bool EXACT>
+__global__ void __launch_bounds__(256, 3)
 embedding_fwd_kernel(const void* __restrict__ tokens, int wide, long long n, const T* __restrict__ weight, long long ld,
                      long long vocab, int dim, float scale, T* __restrict__ out, int segments, int* status) {
-    typedef typename MgwRaw<VEC * sizeof(T)>::type Raw;
-    constexpr int U = lookup_unroll(VEC * (int)sizeof(T));           // vectors that a lane keeps in flight
+    constexpr int N = per_block<T>(), U = lookup_unroll(EXACT);
     const int lane = threadIdx.x & 31;
     const long long warps = (long long)gridDim.x * (blockDim.x >> 5);
-    const int n_vec = dim / VEC;
+    const char* lo = reinterpret_cast<const char*>(weight);
+    const char* hi = reinterpret_cast<const char*>(weight + (vocab - 1) * ld + dim);
     for (long long task = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); task < n * segments; task += warps) {
-        const long long i = task / segments;
+        const long long i = segments == 1 ? task : task / segments;
         const int seg = (int)(task - i * segments);
         const long long t = mgw_token(tokens, wide, i);
-        Raw* dst = reinterpret_cast<Raw*>(out + i * dim);
+        T* dst = out + i * dim;
         const bool valid = t >= 0 && t < vocab;
         if (!valid && lane == 0 && seg == 0) mgw_report_token(status, MGW_OP_EMBEDDING, i, t);
-        const Raw* src = reinterpret_cast<const Raw*>(weight + (valid ? t : 0) * ld);
-        const int c0 = seg * 32 * U + lane;
-        Raw r[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k)
-            if (valid && c0 + 32 * k < n_vec) r[k] = src[c0 + 32 * k];
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            if (c0 + 32 * k >= n_vec) continue;
+        const T* src = weight + (valid ? t : 0) * ld;
+        auto put = [&](uint4 v, int c) {                             // blocks begin on boundaries of the output
             if (!valid || scale != 1.f) {                            // a factor of one copies the bits
-                float f[VEC];
-                if (valid) mgw_unpack<T, VEC>(r[k], f);
+                float f[N];
+                mgw_unpack<T, N>(v, f);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) f[e] = valid ? f[e] * scale : mgw_nan();
-                r[k] = mgw_pack<T, VEC>(f);
+                for (int e = 0; e < N; ++e) f[e] = valid ? f[e] * scale : mgw_nan();
+                v = mgw_pack<T, N>(f);
             }
-            dst[c0 + 32 * k] = r[k];
+            store_block<T, EXACT>(dst, c, dim, v);
+        };
+        const int c = (seg * 32 * U + lane) * N - (EXACT ? 0 : lead_of(dst));
+        if (EXACT || inside(src, dim, lo, hi)) {
+            Cut r[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+                if (c + 32 * N * k < dim) r[k] = load_block<T, EXACT>(src, c + 32 * N * k);
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+                if (c + 32 * N * k < dim) put(take<EXACT>(r[k]), c + 32 * N * k);
+        } else {
+#pragma unroll 1
+            for (int k = 0; k < U; ++k)
+                if (c + 32 * N * k < dim) put(gather_block(src, c + 32 * N * k, dim), c + 32 * N * k);
         }
     }
 }
@@ -233,29 +352,11 @@ struct ClusterSmem {
     uint32_t warp_sum[(1 << kClusterBits) / 32];
 };
 
-// Zeros for a stretch of memory (bytes a multiple of the element size), by blocks [0, blocks).
-__device__ __forceinline__ void fill_zero(char* at, long long bytes, int block, int blocks) {
-    const long long head = min(bytes, (long long)((16 - ((unsigned long long)at & 15)) & 15)), n = (bytes - head) >> 4;
-    uint4* v = reinterpret_cast<uint4*>(at + head);
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (long long i = (long long)block * blockDim.x + threadIdx.x; i < n; i += (long long)blocks * blockDim.x) v[i] = zero;
-    if (block == 0) {
-        if (threadIdx.x < head) at[threadIdx.x] = 0;
-        if (threadIdx.x < bytes - head - (n << 4)) at[head + (n << 4) + threadIdx.x] = 0;
-    }
-}
-
-// The first cluster sorts; the others, if there are any, fill `zeros` meanwhile.
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThreads) sort_cluster_kernel(SortPass p, int passes, char* zeros,
-                                                                                                        long long zero_bytes) {
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThreads) sort_cluster_kernel(SortPass p, int passes) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     ClusterSmem& m = *reinterpret_cast<ClusterSmem*>(dynamic);
     cg::cluster_group cluster = cg::this_cluster();
     mgw_let_next_start();
-    if (blockIdx.x >= kCluster) {
-        fill_zero(zeros, zero_bytes, blockIdx.x - kCluster, gridDim.x - kCluster);
-        return;
-    }
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int bins = 1 << p.bits, n = (int)p.n, rank_in_cluster = (int)cluster.block_rank();
     const int items = (n + kCluster * kClusterThreads - 1) / (kCluster * kClusterThreads);
@@ -344,212 +445,237 @@ struct GradArgs {
     long long vocab;
     int dim;
     float scale;
-    int chunk;                 // entries of the sorted list that one warp adds up
-    int chunks, slabs;         // slab: the columns that a warp covers
-    float* partial;            // [chunks][2][slabs * 32 * NV * VEC]: the run that comes in, the run that goes on
-    int zero_blocks;           // blocks of the launch that fill rows without tokens (0: they are zero already)
+    int chunk;                 // entries of the sorted list that one warp adds up; the 8 warps of a block have neighbouring ones
+    int groups, slabs;         // group: the chunks of a block; slab: 32 blocks of a row, one per lane
+    float* partial;            // [groups][2][slabs * 32 * N]: the run that comes in, the run that goes on
+    int zero_blocks;           // blocks of the launch that fill rows without tokens
+    int zero_rows;             // rows of each of them
+    int by_tokens;             // they look at the tokens themselves (short lists), not at the sorted list
+    const void* tokens;
+    int wide;
+    long long padding;
 };
 
-constexpr int kZeroRows = 8;   // rows that one warp checks and fills
+constexpr int kZeroRows = 1024;            // most rows of a block that fills
 
-// Columns of a lane: NV vectors of VEC elements, 32 vectors apart.
-template <typename T, int VEC, int NV>
-struct Columns {
-    typedef typename MgwRaw<VEC * sizeof(T)>::type Raw;
-    int c[NV];
-    int n_vec;
-    __device__ __forceinline__ Columns(int slab, int lane, int dim) : n_vec(dim / VEC) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k) c[k] = (slab * NV + k) * 32 + lane;
-    }
-    __device__ __forceinline__ void load(const T* row, Raw (&r)[NV]) const {
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (c[k] < n_vec) r[k] = reinterpret_cast<const Raw*>(row)[c[k]];
-    }
-    __device__ __forceinline__ void add(const Raw (&r)[NV], float (&acc)[NV][VEC]) const {
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (c[k] >= n_vec) continue;
-            float f[VEC];
-            mgw_unpack<T, VEC>(r[k], f);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[k][e] += f[e];
-        }
-    }
-    __device__ __forceinline__ void store_row(T* row, float (&acc)[NV][VEC], float scale) const {
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (c[k] >= n_vec) continue;
-            float f[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) f[e] = acc[k][e] * scale;
-            reinterpret_cast<Raw*>(row)[c[k]] = mgw_pack<T, VEC>(f);
-        }
-    }
-};
+constexpr int kSumWarps = 8;
 
-// fp32 partial sums of a slab: the elements of a lane (a multiple of four) one behind the other
-template <int VEC, int NV>
-__device__ __forceinline__ float4* partial_of(const GradArgs& a, long long chunk, int which, int slab, int lane) {
-    static_assert(NV * VEC % 4 == 0, "whole float4s");
-    return reinterpret_cast<float4*>(a.partial) + (((chunk * 2 + which) * a.slabs + slab) * 32 + lane) * (NV * VEC / 4);
+// fp32 partial sums of a slab: the values of a lane one behind the other
+template <typename T>
+__device__ __forceinline__ float4* partial_of(const GradArgs& a, long long group, int which, int slab, int lane) {
+    return reinterpret_cast<float4*>(a.partial) + (((group * 2 + which) * a.slabs + slab) * 32 + lane) * (per_block<T>() / 4);
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void zero_rows(const GradArgs& a, long long block) {
-    typedef typename MgwRaw<VEC * sizeof(T)>::type Raw;
+// A block's rows that no token names.
+template <typename T, bool EXACT>
+__device__ __forceinline__ void fill_rows(const GradArgs& a) {
+    __shared__ uint32_t named[kZeroRows / 32];
+    const long long r0 = (long long)blockIdx.x * a.zero_rows, r1 = min(a.vocab, r0 + a.zero_rows);
+    for (int k = threadIdx.x; k < kZeroRows / 32; k += blockDim.x) named[k] = 0;
+    __syncthreads();
+    if (a.by_tokens) {                                                // needs no order, so the sort may still be running
+        constexpr int U = 8;
+        for (long long i0 = threadIdx.x; i0 < a.n; i0 += blockDim.x * U) {
+            long long t[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) t[u] = i0 + u * blockDim.x < a.n ? mgw_token(a.tokens, a.wide, i0 + u * blockDim.x) : -1;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (t[u] >= r0 && t[u] < r1 && t[u] != a.padding) atomicOr(&named[(t[u] - r0) >> 5], 1u << ((t[u] - r0) & 31));
+        }
+    } else {
+        mgw_wait_for_previous();
+        for (long long r = r0 + threadIdx.x; r < r1; r += blockDim.x) {
+            long long lo = 0, hi = a.n;                               // first entry that is not below the row
+            while (lo < hi) {
+                const long long mid = (lo + hi) >> 1;
+                if (a.list[mid].x < (uint32_t)r) lo = mid + 1; else hi = mid;
+            }
+            if (lo < a.n && a.list[lo].x == (uint32_t)r) atomicOr(&named[(r - r0) >> 5], 1u << ((r - r0) & 31));
+        }
+    }
+    __syncthreads();
     const int lane = threadIdx.x & 31;
-    const long long r0 = (block * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kZeroRows;
-    bool empty = false;
-    if (lane < kZeroRows && r0 + lane < a.vocab) {
-        long long lo = 0, hi = a.n;                                   // first entry that is not below the row
-        while (lo < hi) {
-            const long long mid = (lo + hi) >> 1;
-            if (a.list[mid].x < (uint32_t)(r0 + lane)) lo = mid + 1; else hi = mid;
-        }
-        empty = lo >= a.n || a.list[lo].x != (uint32_t)(r0 + lane);
-    }
-    unsigned todo = __ballot_sync(0xffffffffu, empty);
-    const int n_vec = a.dim / VEC;
-    Raw zero;
-    memset(&zero, 0, sizeof(zero));
-    while (todo) {
-        const int r = __ffs(todo) - 1;
-        todo &= todo - 1;
-        Raw* row = reinterpret_cast<Raw*>(static_cast<T*>(a.dw) + (r0 + r) * a.dim);
-        for (int c = lane; c < n_vec; c += 32) row[c] = zero;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += blockDim.x >> 5) {
+        if (named[(r - r0) >> 5] >> ((r - r0) & 31) & 1) continue;
+        T* row = static_cast<T*>(a.dw) + r * a.dim;
+        for (int c = lane * per_block<T>() - (EXACT ? 0 : lead_of(row)); c < a.dim; c += 32 * per_block<T>())
+            store_block<T, EXACT>(row, c, a.dim, zero);
     }
 }
 
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(256) grad_chunks_kernel(GradArgs a) {
+template <typename T, bool EXACT>
+__global__ void __launch_bounds__(256, EXACT ? 4 : 3) grad_chunks_kernel(GradArgs a) {
     mgw_let_next_start();
-    mgw_wait_for_previous();
     if ((int)blockIdx.x < a.zero_blocks) {
-        zero_rows<T, VEC>(a, blockIdx.x);
+        fill_rows<T, EXACT>(a);
         return;
     }
-    typedef typename MgwRaw<VEC * sizeof(T)>::type Raw;
-    constexpr int U = 4;                                              // rows in flight
-    const int lane = threadIdx.x & 31;
-    const long long task = (long long)(blockIdx.x - a.zero_blocks) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (task >= (long long)a.chunks * a.slabs) return;
-    const long long chunk = task / a.slabs;
-    const int slab = (int)(task - chunk * a.slabs);
-    const Columns<T, VEC, NV> col(slab, lane, a.dim);
+    mgw_wait_for_previous();
+    constexpr int N = per_block<T>(), U = 4;                          // rows in flight
+    __shared__ float parts[kSumWarps][2][N][32];                      // a chunk's run that comes in, its run that goes on
+    __shared__ uint32_t key_first[kSumWarps], key_last[kSumWarps], key_next[kSumWarps + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long group = (blockIdx.x - a.zero_blocks) / a.slabs;
+    const int slab = (int)(blockIdx.x - a.zero_blocks - group * a.slabs), c0 = (slab * 32 + lane) * N;
+    const int c = min(c0, (a.dim - 1) / N * N);                       // lanes behind the row's end read its last block
     const T* dy = static_cast<const T*>(a.dy);
+    const char* lo = static_cast<const char*>(a.dy);
+    const char* hi = reinterpret_cast<const char*>(dy + (a.n - 1) * a.dy_ld + a.dim);
     T* dw = static_cast<T*>(a.dw);
-    const long long i0 = chunk * a.chunk;
-    const long long i1 = i0 + a.chunk < a.n ? i0 + a.chunk : a.n;
-    const uint32_t none = (uint32_t)a.vocab;
-    uint32_t run = a.list[i0].x;
-    if (run == none) return;                                          // nothing but skipped tokens from here on
-    bool comes_in = i0 > 0 && a.list[i0 - 1].x == run;
-    const uint32_t next_key = i1 < a.n ? a.list[i1].x : none;
-    float acc[NV][VEC];
+    const uint32_t none = (uint32_t)a.vocab;                          // key of what is skipped, and of nothing
+    const long long i0 = min(a.n, (group * kSumWarps + warp) * a.chunk), i1 = min(a.n, i0 + a.chunk);
+    const uint32_t first = i0 < i1 ? a.list[i0].x : none, last = i0 < i1 ? a.list[i1 - 1].x : none;
+    const uint32_t before = i0 > 0 && i0 < i1 ? a.list[i0 - 1].x : none, next = i1 < a.n ? a.list[i1].x : none;
+    if (lane == 0) {
+        key_first[warp] = first;
+        key_last[warp] = last;
+        key_next[warp] = next;
+    }
+    uint32_t run = first;
+    bool comes_in = first != none && before == first;
+    float acc[N];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int e = 0; e < N; ++e) acc[e] = 0.f;
+    auto store = [&](uint32_t key) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[k][e] = 0.f;
+        for (int e = 0; e < N; ++e) acc[e] *= a.scale;
+        store_blocks<T, EXACT>(dw + (long long)key * a.dim, c0, a.dim, mgw_pack<T, N>(acc));
+    };
     auto flush = [&](bool goes_on) {
         if (comes_in || goes_on) {
-            float4* to = partial_of<VEC, NV>(a, chunk, comes_in ? 0 : 1, slab, lane);
-            const float* x = &acc[0][0];
 #pragma unroll
-            for (int q = 0; q < NV * VEC / 4; ++q) to[q] = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+            for (int e = 0; e < N; ++e) parts[warp][comes_in ? 0 : 1][e][lane] = acc[e];
         } else {
-            col.store_row(dw + (long long)run * a.dim, acc, a.scale);
+            store(run);
         }
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[k][e] = 0.f;
+        for (int e = 0; e < N; ++e) acc[e] = 0.f;
         comes_in = false;
     };
-    for (long long b0 = i0; b0 < i1; b0 += 32) {                      // 32 entries at a time, one per lane
+    auto add = [&](uint32_t key, const uint4& v) {
+        if (key != run) {
+            flush(false);
+            run = key;
+        }
+        float f[N];
+        mgw_unpack<T, N>(v, f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += f[e];
+    };
+    const bool whole = comes_in && last == first;                     // nothing but the run that comes in
+    for (long long b0 = i0; b0 < i1 && first != none; b0 += 32) {     // 32 entries at a time, one per lane
         const uint2 mine = b0 + lane < i1 ? a.list[b0 + lane] : make_uint2(none, 0u);
         const int m = __popc(__ballot_sync(0xffffffffu, mine.x != none));
-        for (int j = 0; j < m; j += U) {
-            Raw r[U][NV];
+        // rows at the ends of dy, whose blocks cannot be cut out of vectors
+        const bool edge = !EXACT && lane < m && !inside(dy + (long long)mine.y * a.dy_ld, a.dim, lo, hi);
+        const unsigned edges = EXACT ? 0u : __ballot_sync(0xffffffffu, edge);
+        for (int j = 0; j < m; ) {
+            if (j + U <= m && (edges >> j & ((1u << U) - 1u)) == 0) {
+                Cut r[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t p = __shfl_sync(0xffffffffu, mine.y, (j + u) & 31);
-                if (j + u < m) col.load(dy + (long long)p * a.dy_ld, r[u]);
-            }
+                for (int u = 0; u < U; ++u)
+                    r[u] = load_block<T, EXACT>(dy + (long long)__shfl_sync(0xffffffffu, mine.y, j + u) * a.dy_ld, c);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t k = __shfl_sync(0xffffffffu, mine.x, (j + u) & 31);
-                if (j + u < m) {
-                    if (k != run) {
-                        flush(false);
-                        run = k;
-                    }
-                    col.add(r[u], acc);
-                }
+                for (int u = 0; u < U; ++u) add(__shfl_sync(0xffffffffu, mine.x, j + u), take<EXACT>(r[u]));
+                j += U;
+            } else {
+                const T* row = dy + (long long)__shfl_sync(0xffffffffu, mine.y, j) * a.dy_ld;
+                const uint32_t key = __shfl_sync(0xffffffffu, mine.x, j);
+                add(key, gather_block(row, c, a.dim));
+                ++j;
             }
         }
         if (m < 32) break;
     }
-    flush(next_key == run);
+    const bool goes_on = run != none && last == run && next == run;
+    if (run != none) flush(goes_on);
+    __syncthreads();
+    // Runs that cross borders within the block: the warp in which a run starts adds up the parts in their order (and the
+    // first warp those of the run that comes into the block).  What crosses the block's border goes to memory.
+    auto follow = [&](uint32_t key, int from) {                       // adds the parts behind chunk `from`; true: the run ends here
+        for (int w = from; ; ++w) {
+            if (!(key_last[w] == key && key_next[w] == key)) return true;
+            if (w + 1 == kSumWarps) return false;
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] += parts[w + 1][0][e][lane];
+        }
+    };
+    auto keep = [&](int which) {
+        float4* to = partial_of<T>(a, group, which, slab, lane);
+#pragma unroll
+        for (int q = 0; q < N / 4; ++q) to[q] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+    };
+    if (warp == 0 && first != none && before == first) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = parts[0][0][e][lane];
+        follow(first, 0);
+        keep(0);
+    }
+    if (goes_on && !whole) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = parts[warp][1][e][lane];
+        if (follow(last, warp)) store(last);
+        else keep(1);
+    }
 }
 
-// Runs that cross borders of chunks: the warp of the chunk in which a run starts adds up the partial sums.
-template <typename T, int VEC, int NV>
+// Runs that cross borders of groups: the warp of the group in which a run starts adds up its partial sums, for one slab.
+template <typename T, bool EXACT>
 __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a) {
+    constexpr int N = per_block<T>(), Q = N / 4, U = 8;               // partial sums in flight, added in their order
     mgw_wait_for_previous();
     const int lane = threadIdx.x & 31;
-    const long long task = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (task >= (long long)(a.chunks - 1) * a.slabs) return;
-    const long long chunk = task / a.slabs;
-    const int slab = (int)(task - chunk * a.slabs);
-    const long long i0 = chunk * a.chunk, i1 = i0 + a.chunk;          // not the last chunk: it is full
-    const uint32_t run = a.list[i1 - 1].x;
-    if (run == (uint32_t)a.vocab || a.list[i1].x != run) return;
-    if (i0 > 0 && a.list[i0 - 1].x == run) return;                      // it started further left
-    long long end = chunk + 1;                                        // the run's first chunk that is not its own
+    const long long task = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (task >= (long long)(a.groups - 1) * a.slabs) return;
+    const long long group = task / a.slabs, size = (long long)kSumWarps * a.chunk;
+    const int slab = (int)(task - group * a.slabs);
+    const uint32_t none = (uint32_t)a.vocab;
+    const long long i0 = group * size, i1 = i0 + size;                // not the last group: it is full
+    // where the run that crosses the group's end started: in this group if the group has another key or it does not come in
+    const uint32_t run = a.list[i1 - 1].x, next = a.list[i1].x, first = a.list[i0].x, before = i0 > 0 ? a.list[i0 - 1].x : none;
+    if (run == none || next != run || (first == run && before == run)) return;
+    long long end = group + 1;                                        // the run's first group that is not its own
     for (bool more = true; more; ) {
-        const long long c = end + lane;
-        const unsigned same = __ballot_sync(0xffffffffu, c < a.chunks && a.list[c * a.chunk].x == run);
+        const long long g = end + lane;
+        const unsigned same = __ballot_sync(0xffffffffu, g < a.groups && a.list[g * size].x == run);
         const int k = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
         end += k;
         more = k == 32;
     }
-    constexpr int Q = NV * VEC / 4, U = 8;                            // partial sums in flight, added in their order
     float4 x[Q];
-    const float4* from = partial_of<VEC, NV>(a, chunk, 1, slab, lane);
+    const float4* from = partial_of<T>(a, group, 1, slab, lane);
 #pragma unroll
     for (int q = 0; q < Q; ++q) x[q] = from[q];
     const long long step = 2LL * a.slabs * 32 * Q;
-    from = partial_of<VEC, NV>(a, chunk + 1, 0, slab, lane);
-    for (long long c = chunk + 1; c < end; c += U, from += U * step) {
+    from = partial_of<T>(a, group + 1, 0, slab, lane);
+    for (long long g = group + 1; g < end; g += U, from += U * step) {
         float4 y[U][Q];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int q = 0; q < Q; ++q) y[u][q] = c + u < end ? from[u * step + q] : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int q = 0; q < Q; ++q) y[u][q] = g + u < end ? from[u * step + q] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int q = 0; q < Q; ++q) { x[q].x += y[u][q].x; x[q].y += y[u][q].y; x[q].z += y[u][q].z; x[q].w += y[u][q].w; }
     }
-    float acc[NV][VEC];
+    float acc[N];
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-        float* to = &acc[0][0] + 4 * q;
-        to[0] = x[q].x; to[1] = x[q].y; to[2] = x[q].z; to[3] = x[q].w;
+        acc[4 * q] = x[q].x * a.scale; acc[4 * q + 1] = x[q].y * a.scale;
+        acc[4 * q + 2] = x[q].z * a.scale; acc[4 * q + 3] = x[q].w * a.scale;
     }
-    const Columns<T, VEC, NV> col(slab, lane, a.dim);
-    col.store_row(static_cast<T*>(a.dw) + (long long)run * a.dim, acc, a.scale);
+    store_blocks<T, EXACT>(static_cast<T*>(a.dw) + (long long)run * a.dim, (slab * 32 + lane) * N, a.dim, mgw_pack<T, N>(acc));
 }
 
 int element_size(int dtype) { return dtype == MGW_F32 ? 4 : 2; }
 
-// Widest access in bytes that every row of a matrix allows: 16, 4 or one element.
-int access_bytes(const void* base, long long ld, int dim, int dtype) {
+// All rows begin on 16-byte boundaries and consist of whole blocks.
+bool whole_blocks(const void* base, long long ld, int dim, int dtype) {
     const int es = element_size(dtype);
-    const unsigned long long a = (unsigned long long)(uintptr_t)base | (unsigned long long)(ld * es) | (unsigned long long)((long long)dim * es);
-    return (a & 15) == 0 ? 16 : (a & 3) == 0 ? 4 : es;
+    return (((unsigned long long)(uintptr_t)base | (unsigned long long)(ld * es) | (unsigned long long)((long long)dim * es)) & 15) == 0;
 }
 
 // The sort: digits per pass and scratch memory.
@@ -577,43 +703,37 @@ SortPlan sort_plan(long long n, long long vocab) {
 }
 
 struct SumPlan {
-    int vec, nv, slabs, chunk, chunks;
+    int slabs, chunk, groups;
     size_t partial_bytes;
 };
 
-SumPlan sum_plan(long long n, int dim, int dtype, int bytes) {
+SumPlan sum_plan(long long n, int dim, int dtype) {
     SumPlan s;
-    const int es = element_size(dtype);
-    s.vec = bytes / es;
-    s.nv = s.vec >= 4 ? 1 : es == 2 && s.vec == 1 ? 8 : 4;            // narrow accesses: several per lane and row
-    const int n_vec = dim / s.vec;
-    s.slabs = (n_vec + 32 * s.nv - 1) / (32 * s.nv);
+    const int per = 16 / element_size(dtype);
+    s.slabs = (dim + 32 * per - 1) / (32 * per);
     // a warp's part of the list: long enough that partial sums are few, short enough that there are warps for every SM
     s.chunk = 8;
     while (s.chunk < 512 && (n / s.chunk) * s.slabs > 148LL * 64) s.chunk *= 2;
-    s.chunks = (int)((n + s.chunk - 1) / s.chunk);
-    s.partial_bytes = (size_t)s.chunks * 2 * s.slabs * 32 * s.nv * s.vec * sizeof(float);
+    s.groups = (int)((n + (long long)kSumWarps * s.chunk - 1) / ((long long)kSumWarps * s.chunk));
+    s.partial_bytes = (size_t)s.groups * 2 * s.slabs * 32 * per * sizeof(float);
     return s;
 }
 
-template <typename T, int VEC, int NV>
+template <typename T, bool EXACT>
 int launch_sums(const GradArgs& a, cudaStream_t stream) {
-    const long long tasks = (long long)a.chunks * a.slabs;
-    const long long blocks = (tasks + 7) / 8 + a.zero_blocks;
-    const int rc = launch_dependent(grad_chunks_kernel<T, VEC, NV>, blocks, 256, 0, stream, a);
-    if (rc != MGW_OK || a.chunks == 1) return rc;
-    return launch_dependent(grad_join_kernel<T, VEC, NV>, ((long long)(a.chunks - 1) * a.slabs + 7) / 8, 256, 0, stream, a);
+    const int rc = launch_dependent(grad_chunks_kernel<T, EXACT>, (long long)a.groups * a.slabs + a.zero_blocks, 32 * kSumWarps, 0, stream, a);
+    if (rc != MGW_OK || a.groups == 1) return rc;
+    return launch_dependent(grad_join_kernel<T, EXACT>, ((long long)(a.groups - 1) * a.slabs + 7) / 8, 256, 0, stream, a);
 }
 
-template <typename T, int VEC>
+template <typename T, bool EXACT>
 int launch_fwd(const void* tokens, int wide, long long n, const void* weight, long long ld, long long vocab, int dim, float scale,
                void* out, int* status, cudaStream_t stream) {
-    const int n_vec = dim / VEC;
-    const int per = 32 * lookup_unroll(VEC * (int)sizeof(T)), segments = (n_vec + per - 1) / per;
+    const int per = 32 * lookup_unroll(EXACT) * per_block<T>(), segments = (dim + (EXACT ? 0 : per_block<T>() - 1) + per - 1) / per;
     const long long blocks = (n * segments + 7) / 8;
     const unsigned grid = (unsigned)(blocks < 148LL * 64 ? blocks : 148LL * 64);
-    embedding_fwd_kernel<T, VEC><<<grid, 256, 0, stream>>>(tokens, wide, n, static_cast<const T*>(weight), ld, vocab, dim, scale,
-                                                           static_cast<T*>(out), segments, status);
+    embedding_fwd_kernel<T, EXACT><<<grid, 256, 0, stream>>>(tokens, wide, n, static_cast<const T*>(weight), ld, vocab, dim, scale,
+                                                             static_cast<T*>(out), segments, status);
     MGW_CUDA_CHECK(cudaGetLastError());
     return MGW_OK;
 }
@@ -650,27 +770,19 @@ extern "C" int mgw_embedding_fwd(const void* tokens, int wide, long long n, cons
     if (bad_sizes(n, vocab, dim, dtype) || ld < dim) return MGW_ERR_ARG;
     if (n == 0) return MGW_OK;
     if (tokens == nullptr || weight == nullptr || out == nullptr || status == nullptr) return MGW_ERR_ARG;
-    const int wb = access_bytes(weight, ld, dim, dtype), ob = access_bytes(out, dim, dim, dtype);
-    const int bytes = wb < ob ? wb : ob;
+    if (((uintptr_t)weight | (uintptr_t)out) & (element_size(dtype) - 1)) return MGW_ERR_ARG;
+    const bool exact = whole_blocks(weight, ld, dim, dtype) && whole_blocks(out, dim, dim, dtype);
     cudaStream_t s = (cudaStream_t)stream;
-#define MGW_FWD(T, V) launch_fwd<T, V>(tokens, wide, n, weight, ld, vocab, dim, scale, out, status, s)
-    if (dtype == MGW_F32) return bytes == 16 ? MGW_FWD(float, 4) : MGW_FWD(float, 1);
-    if (dtype == MGW_F16) return bytes == 16 ? MGW_FWD(__half, 8) : bytes == 4 ? MGW_FWD(__half, 2) : MGW_FWD(__half, 1);
-    return bytes == 16 ? MGW_FWD(__nv_bfloat16, 8) : bytes == 4 ? MGW_FWD(__nv_bfloat16, 2) : MGW_FWD(__nv_bfloat16, 1);
+#define MGW_FWD(T) (exact ? launch_fwd<T, true>(tokens, wide, n, weight, ld, vocab, dim, scale, out, status, s) \
+                          : launch_fwd<T, false>(tokens, wide, n, weight, ld, vocab, dim, scale, out, status, s))
+    return dtype == MGW_F32 ? MGW_FWD(float) : dtype == MGW_F16 ? MGW_FWD(__half) : MGW_FWD(__nv_bfloat16);
 #undef MGW_FWD
 }
 
 extern "C" size_t mgw_embedding_grad_bytes(long long n, long long vocab, int dim, int dtype) {
     if (bad_sizes(n, vocab, dim, dtype) || n == 0) return 0;
     const SortPlan p = sort_plan(n, vocab);
-    size_t most = 0;                                                  // whatever access width the call ends up with
-    const int es = element_size(dtype);
-    for (int bytes : {16, 4, es}) {
-        if ((long long)dim * es % bytes) continue;
-        const SumPlan s = sum_plan(n, dim, dtype, bytes);
-        if (s.partial_bytes > most) most = s.partial_bytes;
-    }
-    return 2 * p.list_bytes + p.counts_bytes + p.totals_bytes + most;
+    return 2 * p.list_bytes + p.counts_bytes + p.totals_bytes + sum_plan(n, dim, dtype).partial_bytes;
 }
 
 extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* tokens, int wide, long long n, long long vocab, int dim,
@@ -684,10 +796,9 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
     }
     if (dy == nullptr || tokens == nullptr || work == nullptr || status == nullptr || (n > 1 && dy_ld < dim)) return MGW_ERR_ARG;
     if (work_bytes < mgw_embedding_grad_bytes(n, vocab, dim, dtype) || ((uintptr_t)work & 15)) return MGW_ERR_ARG;
+    if (((uintptr_t)dy | (uintptr_t)dw) & (element_size(dtype) - 1)) return MGW_ERR_ARG;
     const SortPlan p = sort_plan(n, vocab);
-    const int db = access_bytes(dy, dy_ld, dim, dtype), wb = access_bytes(dw, dim, dim, dtype);
-    const int bytes = db < wb ? db : wb;
-    const SumPlan q = sum_plan(n, dim, dtype, bytes);
+    const SumPlan q = sum_plan(n, dim, dtype);
     char* at = static_cast<char*>(work);
     uint2* list[2];
     for (int i = 0; i < 2; ++i) {
@@ -696,10 +807,6 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
     }
     uint32_t* counts = reinterpret_cast<uint32_t*>(at); at += p.counts_bytes;
     uint32_t* totals = reinterpret_cast<uint32_t*>(at); at += p.totals_bytes;
-    // Rows without tokens: at most n rows have one.  With n below the vocabulary everything is filled with zeros while the
-    // one cluster sorts (rows with tokens are written twice); with more tokens most rows have one, and the launch that adds
-    // up looks for those that have none.
-    const bool zero_first = n <= kClusterList && n < vocab;
     SortPass a = {};
     a.tokens = tokens; a.wide = wide; a.out = list[0];
     a.counts = counts; a.totals = totals;
@@ -707,8 +814,7 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
     a.vocab = vocab; a.padding = padding; a.status = status;
     if (n <= kClusterList) {
         MGW_CUDA_CHECK(cudaFuncSetAttribute(sort_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSmem)));
-        sort_cluster_kernel<<<zero_first ? 16 * kCluster : kCluster, kClusterThreads, sizeof(ClusterSmem), s>>>(
-            a, p.passes, static_cast<char*>(dw), (long long)vocab * dim * element_size(dtype));
+        sort_cluster_kernel<<<kCluster, kClusterThreads, sizeof(ClusterSmem), s>>>(a, p.passes);
         MGW_CUDA_CHECK(cudaGetLastError());
     } else {
         const int bins = 1 << p.bits;
@@ -726,12 +832,18 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
     GradArgs g;
     g.list = list[n > kClusterList ? (p.passes - 1) & 1 : 0];
     g.n = n; g.dy = dy; g.dy_ld = dy_ld; g.dw = dw; g.vocab = vocab; g.dim = dim; g.scale = scale;
-    g.chunk = q.chunk; g.chunks = q.chunks; g.slabs = q.slabs;
+    g.chunk = q.chunk; g.groups = q.groups; g.slabs = q.slabs;
     g.partial = reinterpret_cast<float*>(at);
-    g.zero_blocks = zero_first ? 0 : (int)((vocab + 8 * kZeroRows - 1) / (8 * kZeroRows));
-    if (dtype == MGW_F32) return bytes == 16 ? launch_sums<float, 4, 1>(g, s) : launch_sums<float, 1, 4>(g, s);
-    if (dtype == MGW_F16)
-        return bytes == 16 ? launch_sums<__half, 8, 1>(g, s) : bytes == 4 ? launch_sums<__half, 2, 4>(g, s) : launch_sums<__half, 1, 8>(g, s);
-    return bytes == 16 ? launch_sums<__nv_bfloat16, 8, 1>(g, s)
-                       : bytes == 4 ? launch_sums<__nv_bfloat16, 2, 4>(g, s) : launch_sums<__nv_bfloat16, 1, 8>(g, s);
+    // Rows without tokens are filled by blocks of the same launch as the sums.  Those of a short list read all tokens and
+    // start while the sort runs; a long list (where every block would read too much) is searched when it is sorted.
+    g.by_tokens = n <= kClusterList;
+    g.tokens = tokens; g.wide = wide; g.padding = padding;
+    const int fillers = !g.by_tokens || n <= 4096 ? 148 * 4 : 148;
+    g.zero_rows = (int)((vocab + fillers - 1) / fillers);
+    if (g.zero_rows > kZeroRows) g.zero_rows = kZeroRows;
+    g.zero_blocks = (int)((vocab + g.zero_rows - 1) / g.zero_rows);
+    const bool exact = whole_blocks(dy, dy_ld, dim, dtype) && whole_blocks(dw, dim, dim, dtype);
+    if (dtype == MGW_F32) return exact ? launch_sums<float, true>(g, s) : launch_sums<float, false>(g, s);
+    if (dtype == MGW_F16) return exact ? launch_sums<__half, true>(g, s) : launch_sums<__half, false>(g, s);
+    return exact ? launch_sums<__nv_bfloat16, true>(g, s) : launch_sums<__nv_bfloat16, false>(g, s);
 }
