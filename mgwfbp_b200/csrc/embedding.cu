@@ -344,6 +344,7 @@ constexpr int kClusterItems = 8;
 constexpr int kClusterPart = kClusterThreads * kClusterItems;         // entries of a block
 constexpr int kClusterList = kCluster * kClusterPart;
 constexpr int kClusterBits = 9;
+constexpr long long kOneBlock = 2048;                                 // up to here one block sorts alone
 
 struct ClusterSmem {
     uint2 list[2][kClusterPart];                                      // {key, position}, before and after a pass
@@ -352,14 +353,14 @@ struct ClusterSmem {
     uint32_t warp_sum[(1 << kClusterBits) / 32];
 };
 
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThreads) sort_cluster_kernel(SortPass p, int passes) {
+__global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(SortPass p, int passes) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     ClusterSmem& m = *reinterpret_cast<ClusterSmem*>(dynamic);
     cg::cluster_group cluster = cg::this_cluster();
     mgw_let_next_start();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int bins = 1 << p.bits, n = (int)p.n, rank_in_cluster = (int)cluster.block_rank();
-    const int items = (n + kCluster * kClusterThreads - 1) / (kCluster * kClusterThreads);
+    const int bins = 1 << p.bits, n = (int)p.n, rank_in_cluster = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks();
+    const int items = (n + blocks * kClusterThreads - 1) / (blocks * kClusterThreads);
     const int part = items * kClusterThreads;                         // entries of a block (of the last ones: fewer)
     const int first = rank_in_cluster * part;
     for (int pass = 0; pass < passes; ++pass) {
@@ -396,14 +397,20 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThrea
             }
             m.hist[tid] = sum;
         }
-        cluster.sync();
+        if (blocks == 1) __syncthreads(); else cluster.sync();
         uint32_t before = 0, total = 0, s = 0;
         if (tid < bins) {
+            if (blocks == 1) {
+                total = m.hist[tid];
+            } else {
+                uint32_t h[kCluster];
 #pragma unroll
-            for (int c = 0; c < kCluster; ++c) {
-                const uint32_t h = cluster.map_shared_rank(m.hist, c)[tid];
-                if (c < rank_in_cluster) before += h;
-                total += h;
+                for (int c = 0; c < kCluster; ++c) h[c] = cluster.map_shared_rank(m.hist, c)[tid];
+#pragma unroll
+                for (int c = 0; c < kCluster; ++c) {
+                    if (c < rank_in_cluster) before += h[c];
+                    total += h[c];
+                }
             }
             s = total;
         }
@@ -427,11 +434,15 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThrea
             if (pass == passes - 1) {
                 p.out[at] = e[j];
             } else {
-                const uint32_t c = at / (uint32_t)part;
-                cluster.map_shared_rank(m.list[to], c)[at - c * part] = e[j];
+                if (blocks == 1) {
+                    m.list[to][at] = e[j];
+                } else {
+                    const uint32_t c = at / (uint32_t)part;
+                    cluster.map_shared_rank(m.list[to], c)[at - c * part] = e[j];
+                }
             }
         }
-        cluster.sync();                                               // the list is in its new order; histograms are free
+        if (blocks == 1) __syncthreads(); else cluster.sync();        // the list is in its new order; histograms are free
     }
 }
 
@@ -459,6 +470,7 @@ struct GradArgs {
 constexpr int kZeroRows = 1024;            // most rows of a block that fills
 
 constexpr int kSumWarps = 8;
+constexpr int kMaxChunk = 64;
 
 // fp32 partial sums of a slab: the values of a lane one behind the other
 template <typename T>
@@ -711,9 +723,10 @@ SumPlan sum_plan(long long n, int dim, int dtype) {
     SumPlan s;
     const int per = 16 / element_size(dtype);
     s.slabs = (dim + 32 * per - 1) / (32 * per);
-    // a warp's part of the list: long enough that partial sums are few, short enough that there are warps for every SM
-    s.chunk = 8;
-    while (s.chunk < 512 && (n / s.chunk) * s.slabs > 148LL * 64) s.chunk *= 2;
+    // A warp's part of the list: short enough that there are blocks for every SM, long enough that they run as one wave
+    // where that is possible (three or four of them per SM) and that few runs cross its borders.
+    const long long even = (n * s.slabs + kSumWarps * 148 * 4 - 1) / (kSumWarps * 148 * 4);
+    s.chunk = (int)(even < 8 ? 8 : even > kMaxChunk ? kMaxChunk : (even + 3) / 4 * 4);
     s.groups = (int)((n + (long long)kSumWarps * s.chunk - 1) / ((long long)kSumWarps * s.chunk));
     s.partial_bytes = (size_t)s.groups * 2 * s.slabs * 32 * per * sizeof(float);
     return s;
@@ -814,8 +827,17 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
     a.vocab = vocab; a.padding = padding; a.status = status;
     if (n <= kClusterList) {
         MGW_CUDA_CHECK(cudaFuncSetAttribute(sort_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSmem)));
-        sort_cluster_kernel<<<kCluster, kClusterThreads, sizeof(ClusterSmem), s>>>(a, p.passes);
-        MGW_CUDA_CHECK(cudaGetLastError());
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(n <= kOneBlock ? 1 : kCluster);
+        cfg.blockDim = dim3(kClusterThreads);
+        cfg.dynamicSmemBytes = sizeof(ClusterSmem);
+        cfg.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = kCluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = n <= kOneBlock ? 0 : 1;
+        MGW_CUDA_CHECK(cudaLaunchKernelEx(&cfg, sort_cluster_kernel, a, p.passes));
     } else {
         const int bins = 1 << p.bits;
         const size_t hist_smem = (size_t)bins * 4, scatter_smem = (size_t)bins * 4 + (size_t)bins * 2 * (kSortThreads / 32);
