@@ -8,6 +8,7 @@
 // that lies inside a chunk is stored at once; a run that crosses a border leaves fp32 partial sums, which a second kernel
 // adds up in the order of the chunks.  Rows that no token names are filled with zeros by the same launch.
 #include <cooperative_groups.h>
+#include <atomic>
 #include <mutex>
 #include "api.h"
 #include "dtypes.cuh"
@@ -344,7 +345,6 @@ constexpr int kClusterItems = 8;
 constexpr int kClusterPart = kClusterThreads * kClusterItems;         // entries of a block
 constexpr int kClusterList = kCluster * kClusterPart;
 constexpr int kClusterBits = 9;
-constexpr long long kOneBlock = 2048;                                 // up to here one block sorts alone
 
 struct ClusterSmem {
     uint2 list[2][kClusterPart];                                      // {key, position}, before and after a pass
@@ -353,14 +353,14 @@ struct ClusterSmem {
     uint32_t warp_sum[(1 << kClusterBits) / 32];
 };
 
-__global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(SortPass p, int passes) {
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThreads) sort_cluster_kernel(SortPass p, int passes) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     ClusterSmem& m = *reinterpret_cast<ClusterSmem*>(dynamic);
     cg::cluster_group cluster = cg::this_cluster();
     mgw_let_next_start();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int bins = 1 << p.bits, n = (int)p.n, rank_in_cluster = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks();
-    const int items = (n + blocks * kClusterThreads - 1) / (blocks * kClusterThreads);
+    const int bins = 1 << p.bits, n = (int)p.n, rank_in_cluster = (int)cluster.block_rank();
+    const int items = (n + kCluster * kClusterThreads - 1) / (kCluster * kClusterThreads);
     const int part = items * kClusterThreads;                         // entries of a block (of the last ones: fewer)
     const int first = rank_in_cluster * part;
     for (int pass = 0; pass < passes; ++pass) {
@@ -397,20 +397,16 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(SortPass 
             }
             m.hist[tid] = sum;
         }
-        if (blocks == 1) __syncthreads(); else cluster.sync();
+        cluster.sync();
         uint32_t before = 0, total = 0, s = 0;
         if (tid < bins) {
-            if (blocks == 1) {
-                total = m.hist[tid];
-            } else {
-                uint32_t h[kCluster];
+            uint32_t h[kCluster];
 #pragma unroll
-                for (int c = 0; c < kCluster; ++c) h[c] = cluster.map_shared_rank(m.hist, c)[tid];
+            for (int c = 0; c < kCluster; ++c) h[c] = cluster.map_shared_rank(m.hist, c)[tid];
 #pragma unroll
-                for (int c = 0; c < kCluster; ++c) {
-                    if (c < rank_in_cluster) before += h[c];
-                    total += h[c];
-                }
+            for (int c = 0; c < kCluster; ++c) {
+                if (c < rank_in_cluster) before += h[c];
+                total += h[c];
             }
             s = total;
         }
@@ -434,16 +430,66 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(SortPass 
             if (pass == passes - 1) {
                 p.out[at] = e[j];
             } else {
-                if (blocks == 1) {
-                    m.list[to][at] = e[j];
-                } else {
-                    const uint32_t c = at / (uint32_t)part;
-                    cluster.map_shared_rank(m.list[to], c)[at - c * part] = e[j];
-                }
+                const uint32_t c = at / (uint32_t)part;
+                cluster.map_shared_rank(m.list[to], c)[at - c * part] = e[j];
             }
         }
-        if (blocks == 1) __syncthreads(); else cluster.sync();        // the list is in its new order; histograms are free
+        cluster.sync();                                               // the list is in its new order; histograms are free
     }
+}
+
+// The same within one block of 1024 threads, for at most 1024 tokens, one per thread; the sorted list is left in shared memory.
+constexpr int kSmallWarps = 32;
+constexpr int kSmallList = kSmallWarps * 32;                          // up to here one launch does it all
+
+struct SmallSort {
+    uint16_t cnt[kSmallWarps][1 << kClusterBits];
+    uint32_t base[1 << kClusterBits], warp_sum[(1 << kClusterBits) / 32];
+};
+
+__device__ __forceinline__ const uint2* sort_in_block(const SortPass& p, int passes, uint2 (*list)[kSmallList], SmallSort& m) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << p.bits, n = (int)p.n;
+    const bool in = tid < n;
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * p.bits;
+        for (int b = tid; b < bins * kSmallWarps; b += kSmallWarps * 32) m.cnt[b >> p.bits][b & (bins - 1)] = 0;
+        uint2 e = make_uint2(0, 0);
+        if (in) e = pass == 0 ? sort_entry(p, tid, true) : list[(pass + 1) & 1][tid];
+        const uint32_t d = in ? (e.x >> shift) & (bins - 1) : 0xffffffffu;
+        __syncthreads();
+        const unsigned peers = __match_any_sync(0xffffffffu, d);
+        const uint32_t rank = __popc(peers & ((1u << lane) - 1u));
+        if (in && lane == 31 - __clz(peers)) m.cnt[warp][d] = (uint16_t)(rank + 1);
+        __syncthreads();
+        uint32_t total = 0, s = 0;
+        if (tid < bins) {                                             // a digit's entries in the warps before, and in all
+            uint32_t c[kSmallWarps];
+#pragma unroll
+            for (int w = 0; w < kSmallWarps; ++w) c[w] = m.cnt[w][tid];
+#pragma unroll
+            for (int w = 0; w < kSmallWarps; ++w) {
+                m.cnt[w][tid] = (uint16_t)total;
+                total += c[w];
+            }
+        }
+        s = total;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += v;
+        }
+        if (lane == 31 && warp < (1 << kClusterBits) / 32) m.warp_sum[warp] = s;
+        __syncthreads();
+        if (tid < bins) {
+            uint32_t before = 0;
+            for (int w = 0; w < warp; ++w) before += m.warp_sum[w];
+            m.base[tid] = before + s - total;
+        }
+        __syncthreads();
+        if (in) list[pass & 1][m.base[d] + m.cnt[warp][d] + rank] = e;
+        __syncthreads();
+    }
+    return list[(passes - 1) & 1];
 }
 
 // -------------------------------------------------------------------------------------------------------------- sums
@@ -480,9 +526,9 @@ __device__ __forceinline__ float4* partial_of(const GradArgs& a, long long group
 
 // A block's rows that no token names.
 template <typename T, bool EXACT>
-__device__ __forceinline__ void fill_rows(const GradArgs& a) {
+__device__ __forceinline__ void fill_rows(const GradArgs& a, long long block) {
     __shared__ uint32_t named[kZeroRows / 32];
-    const long long r0 = (long long)blockIdx.x * a.zero_rows, r1 = min(a.vocab, r0 + a.zero_rows);
+    const long long r0 = block * a.zero_rows, r1 = min(a.vocab, r0 + a.zero_rows);
     for (int k = threadIdx.x; k < kZeroRows / 32; k += blockDim.x) named[k] = 0;
     __syncthreads();
     if (a.by_tokens) {                                                // needs no order, so the sort may still be running
@@ -517,33 +563,30 @@ __device__ __forceinline__ void fill_rows(const GradArgs& a) {
     }
 }
 
-template <typename T, bool EXACT>
-__global__ void __launch_bounds__(256, EXACT ? 4 : 3) grad_chunks_kernel(GradArgs a) {
-    mgw_let_next_start();
-    if ((int)blockIdx.x < a.zero_blocks) {
-        fill_rows<T, EXACT>(a);
-        return;
-    }
-    mgw_wait_for_previous();
+// What the warps of a block share: a chunk's run that comes in and its run that goes on, and the keys around the borders.
+template <typename T, int WARPS>
+struct SumSpace {
+    float parts[WARPS][2][per_block<T>()][32];
+    uint32_t key_last[WARPS], key_next[WARPS];
+};
+
+// The chunks of a group, one per warp, for the columns of a slab.
+template <typename T, bool EXACT, int WARPS>
+__device__ __forceinline__ void sum_group(const GradArgs& a, const uint2* list, long long group, int slab, SumSpace<T, WARPS>& m) {
     constexpr int N = per_block<T>(), U = 4;                          // rows in flight
-    __shared__ float parts[kSumWarps][2][N][32];                      // a chunk's run that comes in, its run that goes on
-    __shared__ uint32_t key_first[kSumWarps], key_last[kSumWarps], key_next[kSumWarps + 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long group = (blockIdx.x - a.zero_blocks) / a.slabs;
-    const int slab = (int)(blockIdx.x - a.zero_blocks - group * a.slabs), c0 = (slab * 32 + lane) * N;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = (slab * 32 + lane) * N;
     const int c = min(c0, (a.dim - 1) / N * N);                       // lanes behind the row's end read its last block
     const T* dy = static_cast<const T*>(a.dy);
     const char* lo = static_cast<const char*>(a.dy);
     const char* hi = reinterpret_cast<const char*>(dy + (a.n - 1) * a.dy_ld + a.dim);
     T* dw = static_cast<T*>(a.dw);
     const uint32_t none = (uint32_t)a.vocab;                          // key of what is skipped, and of nothing
-    const long long i0 = min(a.n, (group * kSumWarps + warp) * a.chunk), i1 = min(a.n, i0 + a.chunk);
-    const uint32_t first = i0 < i1 ? a.list[i0].x : none, last = i0 < i1 ? a.list[i1 - 1].x : none;
-    const uint32_t before = i0 > 0 && i0 < i1 ? a.list[i0 - 1].x : none, next = i1 < a.n ? a.list[i1].x : none;
+    const long long i0 = min(a.n, (group * WARPS + warp) * a.chunk), i1 = min(a.n, i0 + a.chunk);
+    const uint32_t first = i0 < i1 ? list[i0].x : none, last = i0 < i1 ? list[i1 - 1].x : none;
+    const uint32_t before = i0 > 0 && i0 < i1 ? list[i0 - 1].x : none, next = i1 < a.n ? list[i1].x : none;
     if (lane == 0) {
-        key_first[warp] = first;
-        key_last[warp] = last;
-        key_next[warp] = next;
+        m.key_last[warp] = last;
+        m.key_next[warp] = next;
     }
     uint32_t run = first;
     bool comes_in = first != none && before == first;
@@ -558,7 +601,7 @@ __global__ void __launch_bounds__(256, EXACT ? 4 : 3) grad_chunks_kernel(GradArg
     auto flush = [&](bool goes_on) {
         if (comes_in || goes_on) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) parts[warp][comes_in ? 0 : 1][e][lane] = acc[e];
+            for (int e = 0; e < N; ++e) m.parts[warp][comes_in ? 0 : 1][e][lane] = acc[e];
         } else {
             store(run);
         }
@@ -578,13 +621,13 @@ __global__ void __launch_bounds__(256, EXACT ? 4 : 3) grad_chunks_kernel(GradArg
     };
     const bool whole = comes_in && last == first;                     // nothing but the run that comes in
     for (long long b0 = i0; b0 < i1 && first != none; b0 += 32) {     // 32 entries at a time, one per lane
-        const uint2 mine = b0 + lane < i1 ? a.list[b0 + lane] : make_uint2(none, 0u);
-        const int m = __popc(__ballot_sync(0xffffffffu, mine.x != none));
+        const uint2 mine = b0 + lane < i1 ? list[b0 + lane] : make_uint2(none, 0u);
+        const int here = __popc(__ballot_sync(0xffffffffu, mine.x != none));
         // rows at the ends of dy, whose blocks cannot be cut out of vectors
-        const bool edge = !EXACT && lane < m && !inside(dy + (long long)mine.y * a.dy_ld, a.dim, lo, hi);
+        const bool edge = !EXACT && lane < here && !inside(dy + (long long)mine.y * a.dy_ld, a.dim, lo, hi);
         const unsigned edges = EXACT ? 0u : __ballot_sync(0xffffffffu, edge);
-        for (int j = 0; j < m; ) {
-            if (j + U <= m && (edges >> j & ((1u << U) - 1u)) == 0) {
+        for (int j = 0; j < here; ) {
+            if (j + U <= here && (edges >> j & ((1u << U) - 1u)) == 0) {
                 Cut r[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -599,7 +642,7 @@ __global__ void __launch_bounds__(256, EXACT ? 4 : 3) grad_chunks_kernel(GradArg
                 ++j;
             }
         }
-        if (m < 32) break;
+        if (here < 32) break;
     }
     const bool goes_on = run != none && last == run && next == run;
     if (run != none) flush(goes_on);
@@ -608,10 +651,10 @@ __global__ void __launch_bounds__(256, EXACT ? 4 : 3) grad_chunks_kernel(GradArg
     // first warp those of the run that comes into the block).  What crosses the block's border goes to memory.
     auto follow = [&](uint32_t key, int from) {                       // adds the parts behind chunk `from`; true: the run ends here
         for (int w = from; ; ++w) {
-            if (!(key_last[w] == key && key_next[w] == key)) return true;
-            if (w + 1 == kSumWarps) return false;
+            if (!(m.key_last[w] == key && m.key_next[w] == key)) return true;
+            if (w + 1 == WARPS) return false;
 #pragma unroll
-            for (int e = 0; e < N; ++e) acc[e] += parts[w + 1][0][e][lane];
+            for (int e = 0; e < N; ++e) acc[e] += m.parts[w + 1][0][e][lane];
         }
     };
     auto keep = [&](int which) {
@@ -621,16 +664,48 @@ __global__ void __launch_bounds__(256, EXACT ? 4 : 3) grad_chunks_kernel(GradArg
     };
     if (warp == 0 && first != none && before == first) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] = parts[0][0][e][lane];
+        for (int e = 0; e < N; ++e) acc[e] = m.parts[0][0][e][lane];
         follow(first, 0);
         keep(0);
     }
     if (goes_on && !whole) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] = parts[warp][1][e][lane];
+        for (int e = 0; e < N; ++e) acc[e] = m.parts[warp][1][e][lane];
         if (follow(last, warp)) store(last);
         else keep(1);
     }
+}
+
+template <typename T, bool EXACT>
+__global__ void __launch_bounds__(32 * kSumWarps, EXACT ? 4 : 3) grad_chunks_kernel(GradArgs a) {
+    __shared__ SumSpace<T, kSumWarps> m;
+    mgw_let_next_start();
+    if ((int)blockIdx.x < a.zero_blocks) {
+        fill_rows<T, EXACT>(a, blockIdx.x);
+        return;
+    }
+    mgw_wait_for_previous();
+    const long long task = blockIdx.x - a.zero_blocks, group = task / a.slabs;
+    sum_group<T, EXACT, kSumWarps>(a, a.list, group, (int)(task - group * a.slabs), m);
+}
+
+// Everything in one launch, for at most 1024 tokens: every slab's block sorts the list for itself and is the only group.
+struct SmallSpace {
+    uint2 list[2][kSmallList];
+    unsigned char rest[];                  // SmallSort, then SumSpace
+};
+
+template <typename T, bool EXACT>
+__global__ void __launch_bounds__(32 * kSmallWarps) grad_small_kernel(GradArgs a, SortPass p, int passes) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    SmallSpace& m = *reinterpret_cast<SmallSpace*>(dynamic);
+    if ((int)blockIdx.x >= a.slabs) {
+        fill_rows<T, EXACT>(a, blockIdx.x - a.slabs);
+        return;
+    }
+    if (blockIdx.x > 0) p.status = nullptr;                           // one report is enough
+    const uint2* list = sort_in_block(p, passes, m.list, *reinterpret_cast<SmallSort*>(m.rest));
+    sum_group<T, EXACT, kSmallWarps>(a, list, 0, blockIdx.x, *reinterpret_cast<SumSpace<T, kSmallWarps>*>(m.rest));
 }
 
 // Runs that cross borders of groups: the warp of the group in which a run starts adds up its partial sums, for one slab.
@@ -732,6 +807,30 @@ SumPlan sum_plan(long long n, int dim, int dtype) {
     return s;
 }
 
+// Lets a kernel use more than 48 KB of shared memory: once for every device.
+template <typename... P>
+int allow_smem(void (*kernel)(P...), size_t bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    MGW_CUDA_CHECK(cudaGetDevice(&dev));
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return MGW_OK;
+    MGW_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return MGW_OK;
+}
+
+template <typename T, bool EXACT>
+int launch_small(const GradArgs& a, const SortPass& p, int passes, cudaStream_t stream) {
+    static std::atomic<unsigned long long> done{0};
+    const size_t rest = sizeof(SmallSort) > sizeof(SumSpace<T, kSmallWarps>) ? sizeof(SmallSort) : sizeof(SumSpace<T, kSmallWarps>);
+    const size_t smem = sizeof(SmallSpace) + rest;
+    const int rc = allow_smem(grad_small_kernel<T, EXACT>, smem, done);
+    if (rc != MGW_OK) return rc;
+    grad_small_kernel<T, EXACT><<<a.slabs + a.zero_blocks, 32 * kSmallWarps, smem, stream>>>(a, p, passes);
+    MGW_CUDA_CHECK(cudaGetLastError());
+    return MGW_OK;
+}
+
 template <typename T, bool EXACT>
 int launch_sums(const GradArgs& a, cudaStream_t stream) {
     const int rc = launch_dependent(grad_chunks_kernel<T, EXACT>, (long long)a.groups * a.slabs + a.zero_blocks, 32 * kSumWarps, 0, stream, a);
@@ -794,6 +893,7 @@ extern "C" int mgw_embedding_fwd(const void* tokens, int wide, long long n, cons
 
 extern "C" size_t mgw_embedding_grad_bytes(long long n, long long vocab, int dim, int dtype) {
     if (bad_sizes(n, vocab, dim, dtype) || n == 0) return 0;
+    if (n <= kSmallList) return 0;
     const SortPlan p = sort_plan(n, vocab);
     return 2 * p.list_bytes + p.counts_bytes + p.totals_bytes + sum_plan(n, dim, dtype).partial_bytes;
 }
@@ -807,37 +907,51 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
         MGW_CUDA_CHECK(cudaMemsetAsync(dw, 0, (size_t)vocab * dim * element_size(dtype), s));
         return MGW_OK;
     }
-    if (dy == nullptr || tokens == nullptr || work == nullptr || status == nullptr || (n > 1 && dy_ld < dim)) return MGW_ERR_ARG;
-    if (work_bytes < mgw_embedding_grad_bytes(n, vocab, dim, dtype) || ((uintptr_t)work & 15)) return MGW_ERR_ARG;
+    if (dy == nullptr || tokens == nullptr || status == nullptr || (n > 1 && dy_ld < dim)) return MGW_ERR_ARG;
     if (((uintptr_t)dy | (uintptr_t)dw) & (element_size(dtype) - 1)) return MGW_ERR_ARG;
     const SortPlan p = sort_plan(n, vocab);
     const SumPlan q = sum_plan(n, dim, dtype);
+    SortPass a = {};
+    a.tokens = tokens; a.wide = wide;
+    a.n = n; a.tiles = p.tiles; a.bits = p.bits;
+    a.vocab = vocab; a.padding = padding; a.status = status;
+    // Rows without tokens are filled by blocks of the same launch as the sums.  Those of a short list read all tokens and
+    // start while the sort runs; a long list (where every block would read too much) is searched when it is sorted.
+    GradArgs g = {};
+    g.n = n; g.dy = dy; g.dy_ld = dy_ld; g.dw = dw; g.vocab = vocab; g.dim = dim; g.scale = scale;
+    g.chunk = q.chunk; g.groups = q.groups; g.slabs = q.slabs;
+    g.by_tokens = n <= kClusterList;
+    g.tokens = tokens; g.wide = wide; g.padding = padding;
+    const bool exact = whole_blocks(dy, dy_ld, dim, dtype) && whole_blocks(dw, dim, dim, dtype);
+    const bool small = n <= kSmallList;
+    const int fillers = small ? (q.slabs < 74 ? 148 - q.slabs : 74) : !g.by_tokens || n <= 4096 ? 148 * 4 : 148;
+    g.zero_rows = (int)((vocab + fillers - 1) / fillers);
+    if (g.zero_rows > kZeroRows) g.zero_rows = kZeroRows;
+    g.zero_blocks = (int)((vocab + g.zero_rows - 1) / g.zero_rows);
+#define MGW_BY_TYPE(f, ...)                                                                            \
+    (dtype == MGW_F32   ? (exact ? f<float, true>(__VA_ARGS__) : f<float, false>(__VA_ARGS__))         \
+     : dtype == MGW_F16 ? (exact ? f<__half, true>(__VA_ARGS__) : f<__half, false>(__VA_ARGS__))       \
+                        : (exact ? f<__nv_bfloat16, true>(__VA_ARGS__) : f<__nv_bfloat16, false>(__VA_ARGS__)))
+    if (small) {
+        g.chunk = (int)((n + kSmallWarps - 1) / kSmallWarps);
+        return MGW_BY_TYPE(launch_small, g, a, p.passes, s);
+    }
+    if (work == nullptr || work_bytes < mgw_embedding_grad_bytes(n, vocab, dim, dtype) || ((uintptr_t)work & 15)) return MGW_ERR_ARG;
     char* at = static_cast<char*>(work);
     uint2* list[2];
     for (int i = 0; i < 2; ++i) {
         list[i] = reinterpret_cast<uint2*>(at);
         at += p.list_bytes;
     }
-    uint32_t* counts = reinterpret_cast<uint32_t*>(at); at += p.counts_bytes;
-    uint32_t* totals = reinterpret_cast<uint32_t*>(at); at += p.totals_bytes;
-    SortPass a = {};
-    a.tokens = tokens; a.wide = wide; a.out = list[0];
-    a.counts = counts; a.totals = totals;
-    a.n = n; a.tiles = p.tiles; a.bits = p.bits;
-    a.vocab = vocab; a.padding = padding; a.status = status;
+    a.out = list[0];
+    a.counts = reinterpret_cast<uint32_t*>(at); at += p.counts_bytes;
+    a.totals = reinterpret_cast<uint32_t*>(at); at += p.totals_bytes;
     if (n <= kClusterList) {
-        MGW_CUDA_CHECK(cudaFuncSetAttribute(sort_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSmem)));
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(n <= kOneBlock ? 1 : kCluster);
-        cfg.blockDim = dim3(kClusterThreads);
-        cfg.dynamicSmemBytes = sizeof(ClusterSmem);
-        cfg.stream = s;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = kCluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = n <= kOneBlock ? 0 : 1;
-        MGW_CUDA_CHECK(cudaLaunchKernelEx(&cfg, sort_cluster_kernel, a, p.passes));
+        static std::atomic<unsigned long long> done{0};
+        const int rc = allow_smem(sort_cluster_kernel, sizeof(ClusterSmem), done);
+        if (rc != MGW_OK) return rc;
+        sort_cluster_kernel<<<kCluster, kClusterThreads, sizeof(ClusterSmem), s>>>(a, p.passes);
+        MGW_CUDA_CHECK(cudaGetLastError());
     } else {
         const int bins = 1 << p.bits;
         const size_t hist_smem = (size_t)bins * 4, scatter_smem = (size_t)bins * 4 + (size_t)bins * 2 * (kSortThreads / 32);
@@ -846,26 +960,13 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
             a.out = list[k & 1];
             a.shift = k * p.bits;
             int rc = launch_dependent(sort_hist_kernel, p.tiles, kSortThreads, hist_smem, s, a);
-            if (rc == MGW_OK) rc = launch_dependent(sort_scan_kernel, (bins + 7) / 8, 256, 0, s, counts, totals, bins, p.tiles);
+            if (rc == MGW_OK) rc = launch_dependent(sort_scan_kernel, (bins + 7) / 8, 256, 0, s, a.counts, a.totals, bins, p.tiles);
             if (rc == MGW_OK) rc = launch_dependent(sort_scatter_kernel, p.tiles, kSortThreads, scatter_smem, s, a);
             if (rc != MGW_OK) return rc;
         }
     }
-    GradArgs g;
     g.list = list[n > kClusterList ? (p.passes - 1) & 1 : 0];
-    g.n = n; g.dy = dy; g.dy_ld = dy_ld; g.dw = dw; g.vocab = vocab; g.dim = dim; g.scale = scale;
-    g.chunk = q.chunk; g.groups = q.groups; g.slabs = q.slabs;
     g.partial = reinterpret_cast<float*>(at);
-    // Rows without tokens are filled by blocks of the same launch as the sums.  Those of a short list read all tokens and
-    // start while the sort runs; a long list (where every block would read too much) is searched when it is sorted.
-    g.by_tokens = n <= kClusterList;
-    g.tokens = tokens; g.wide = wide; g.padding = padding;
-    const int fillers = !g.by_tokens || n <= 4096 ? 148 * 4 : 148;
-    g.zero_rows = (int)((vocab + fillers - 1) / fillers);
-    if (g.zero_rows > kZeroRows) g.zero_rows = kZeroRows;
-    g.zero_blocks = (int)((vocab + g.zero_rows - 1) / g.zero_rows);
-    const bool exact = whole_blocks(dy, dy_ld, dim, dtype) && whole_blocks(dw, dim, dim, dtype);
-    if (dtype == MGW_F32) return exact ? launch_sums<float, true>(g, s) : launch_sums<float, false>(g, s);
-    if (dtype == MGW_F16) return exact ? launch_sums<__half, true>(g, s) : launch_sums<__half, false>(g, s);
-    return exact ? launch_sums<__nv_bfloat16, true>(g, s) : launch_sums<__nv_bfloat16, false>(g, s);
+    return MGW_BY_TYPE(launch_sums, g, s);
+#undef MGW_BY_TYPE
 }

@@ -122,10 +122,10 @@ def _grad_cuda(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: floa
     with device_guard(grad):
         dw = torch.empty(vocab, dim, dtype=grad.dtype, device=grad.device)
         need = _work_bytes(n, vocab, dim, code)
-        work = torch.empty(need, dtype=torch.uint8, device=grad.device)
+        work = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
         _lib.check(_lib_ready().mgw_embedding_grad(rows.data_ptr(), rows.stride(0) if n > 1 else dim, tokens.data_ptr(),
                                                    tokens.dtype == torch.int64, n, vocab, dim, code, scale, padding, dw.data_ptr(),
-                                                   work.data_ptr(), need, status_words(), stream_of(grad)), 'embedding_grad')
+                                                   None if work is None else work.data_ptr(), need, status_words(), stream_of(grad)), 'embedding_grad')
         counters.bump('embedding_grad')
     return dw
 

@@ -212,9 +212,9 @@ def test_native_embedding_refuses_bad_arguments():
     for bad in (dict(tokens=None), dict(weight=None), dict(out=None), dict(status=None), dict(n=-1), dict(n=1 << 31), dict(vocab=0),
                 dict(vocab=(1 << 31) - 1), dict(dim=0), dict(dtype=3), dict(dtype=-1), dict(ld=3)):
         assert lib.mgw_embedding_fwd(*{**ok, **bad}.values()) == 2, bad
-    need = lib.mgw_embedding_grad_bytes(4, 8, 4, 0)
-    assert need > 0 and lib.mgw_embedding_grad_bytes(0, 8, 4, 0) == 0
-    ok = dict(dy=p, ld=4, tokens=p, wide=0, n=4, vocab=8, dim=4, dtype=0, scale=1.0, padding=-1, dw=p, work=p & ~15, bytes=need,
+    need = lib.mgw_embedding_grad_bytes(2000, 8, 4, 0)             # short lists need no scratch memory
+    assert need > 0 and lib.mgw_embedding_grad_bytes(0, 8, 4, 0) == 0 and lib.mgw_embedding_grad_bytes(1024, 8, 4, 0) == 0
+    ok = dict(dy=p, ld=4, tokens=p, wide=0, n=2000, vocab=8, dim=4, dtype=0, scale=1.0, padding=-1, dw=p, work=p & ~15, bytes=need,
               status=p, stream=None)
     for bad in (dict(dy=None), dict(tokens=None), dict(dw=None), dict(work=None), dict(status=None), dict(bytes=need - 1), dict(ld=3),
                 dict(work=(p & ~15) + 8), dict(dtype=7), dict(dim=-1)):
