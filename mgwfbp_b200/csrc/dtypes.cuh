@@ -35,19 +35,41 @@ union MgwVec {
     __device__ __forceinline__ MgwVec() {}
 };
 
+// Two values at a time: one instruction converts a pair, single values take the slow conversion pipe.
+__device__ __forceinline__ float2 mgw_to_float2(const __half* p) { return __half22float2(__halves2half2(p[0], p[1])); }
+__device__ __forceinline__ float2 mgw_to_float2(const __nv_bfloat16* p) { return __bfloat1622float2(__halves2bfloat162(p[0], p[1])); }
+__device__ __forceinline__ float2 mgw_to_float2(const float* p) { return make_float2(p[0], p[1]); }
+__device__ __forceinline__ void mgw_from_float2(__half* p, float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    p[0] = __low2half(h);
+    p[1] = __high2half(h);
+}
+__device__ __forceinline__ void mgw_from_float2(__nv_bfloat16* p, float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    p[0] = __low2bfloat16(h);
+    p[1] = __high2bfloat16(h);
+}
+__device__ __forceinline__ void mgw_from_float2(float* p, float a, float b) { p[0] = a; p[1] = b; }
+
 template <typename T, int N>
 __device__ __forceinline__ void mgw_unpack(const typename MgwRaw<N * sizeof(T)>::type& raw, float (&f)[N]) {
     MgwVec<T, N> u;
     u.raw = raw;
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = mgw_to_float(u.v[i]);
+    for (int i = 0; i + 1 < N; i += 2) {
+        const float2 x = mgw_to_float2(u.v + i);
+        f[i] = x.x;
+        f[i + 1] = x.y;
+    }
+    if (N & 1) f[N - 1] = mgw_to_float(u.v[N - 1]);
 }
 
 template <typename T, int N>
 __device__ __forceinline__ typename MgwRaw<N * sizeof(T)>::type mgw_pack(const float (&f)[N]) {
     MgwVec<T, N> u;
 #pragma unroll
-    for (int i = 0; i < N; ++i) u.v[i] = mgw_from_float<T>(f[i]);
+    for (int i = 0; i + 1 < N; i += 2) mgw_from_float2(u.v + i, f[i], f[i + 1]);
+    if (N & 1) u.v[N - 1] = mgw_from_float<T>(f[N - 1]);
     return u.raw;
 }
 

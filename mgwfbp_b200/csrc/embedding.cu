@@ -93,41 +93,48 @@ __device__ __forceinline__ uint4 take(const Cut& c) {
                       __funnelshift_r(b3, b4, bits));
 }
 
-// The elements of a block whose bits are set, one by one: the ends of a row.  Kept small, it is executed rarely.
-__device__ __forceinline__ void store_element(float* to, const uint4& v, int e) {
-    *to = __uint_as_float(e & 2 ? (e & 1 ? v.w : v.z) : (e & 1 ? v.y : v.x));
-}
-template <typename T>
-__device__ __forceinline__ void store_element(T* to, const uint4& v, int e) {
-    const uint32_t w = e & 4 ? (e & 2 ? v.w : v.z) : (e & 2 ? v.y : v.x);
-    *reinterpret_cast<uint16_t*>(to) = (uint16_t)(e & 1 ? w >> 16 : w);
-}
-template <typename T>
-__device__ __forceinline__ void store_some(T* at, const uint4& v, unsigned which) {
-#pragma unroll 1
-    for (; which != 0; which &= which - 1) {
-        const int e = __ffs(which) - 1;
-        store_element(at + e, v, e);
+// The elements [begin, stop) of a block at a 16-byte boundary: one store for a whole block, else up to three towards the
+// middle and three behind it, each as wide as its place allows.
+__device__ __forceinline__ void store_part(float* at, const uint4& v, int begin, int stop) {
+    if (begin <= 0 && stop >= 4) {
+        __stcs(reinterpret_cast<uint4*>(at), v);
+        return;
     }
+    uint32_t* w = reinterpret_cast<uint32_t*>(at);
+    if (begin <= 0 && 0 < stop) w[0] = v.x;
+    if (begin <= 1 && 1 < stop) w[1] = v.y;
+    if (begin <= 2 && 2 < stop) w[2] = v.z;
+    if (begin <= 3 && 3 < stop) w[3] = v.w;
 }
-// Bits of the elements [from, to) of a block.
-__device__ __forceinline__ unsigned range_bits(int from, int to) {
-    return from >= to ? 0u : ((1u << to) - 1u) & ~((1u << max(from, 0)) - 1u);
+
+template <typename T>
+__device__ __forceinline__ void store_part(T* at, const uint4& v, int begin, int stop) {
+    if (begin <= 0 && stop >= 8) {
+        __stcs(reinterpret_cast<uint4*>(at), v);
+        return;
+    }
+    auto word = [&](int e) { return e & 4 ? (e & 2 ? v.w : v.z) : (e & 2 ? v.y : v.x); };
+    char* p = reinterpret_cast<char*>(at);
+    int e = max(begin, 0);
+    stop = min(stop, 8);
+    if (e & 1 && e < stop) { *reinterpret_cast<uint16_t*>(p + 2 * e) = (uint16_t)(word(e) >> 16); ++e; }
+    if (e & 2 && e + 2 <= stop) { *reinterpret_cast<uint32_t*>(p + 2 * e) = word(e); e += 2; }
+    if (e == 4 && stop == 8) { *reinterpret_cast<uint2*>(p + 8) = make_uint2(v.z, v.w); return; }
+    if (e == 0 && stop >= 4) { *reinterpret_cast<uint2*>(p) = make_uint2(v.x, v.y); e = 4; }
+    if (e + 2 <= stop) { *reinterpret_cast<uint32_t*>(p + 2 * e) = word(e); e += 2; }
+    if (e < stop) *reinterpret_cast<uint16_t*>(p + 2 * e) = (uint16_t)word(e);
 }
 
 // A block that begins on a boundary, or the part of it in [0, dim).
 template <typename T, bool EXACT>
 __device__ __forceinline__ void store_block(T* row, int c0, int dim, const uint4& v) {
-    if (EXACT || (c0 >= 0 && c0 + per_block<T>() <= dim)) {
-        __stcs(reinterpret_cast<uint4*>(row + c0), v);
-        return;
-    }
-    store_some(row + c0, v, range_bits(-c0, min(per_block<T>(), dim - c0)));
+    if (EXACT) __stcs(reinterpret_cast<uint4*>(row + c0), v);
+    else store_part(row + c0, v, -c0, dim - c0);
 }
 
 // A warp's 32 neighbouring blocks, lane's at column c0 (all lanes take part; those with c0 >= dim have nothing).  With the
-// row `lead` elements behind a boundary, a lane puts the last `lead` elements of the lane before it in front of its own; what
-// no vector covers at the ends goes element by element.
+// row `lead` elements behind a boundary, a lane stores the block that begins `lead` before its own: the last elements of
+// the lane before it and its own first ones.
 template <typename T, bool EXACT>
 __device__ __forceinline__ void store_blocks(T* row, int c0, int dim, const uint4& v) {
     constexpr int N = per_block<T>();
@@ -135,19 +142,19 @@ __device__ __forceinline__ void store_blocks(T* row, int c0, int dim, const uint
         if (c0 < dim) __stcs(reinterpret_cast<uint4*>(row + c0), v);
         return;
     }
-    const int lane = threadIdx.x & 31, lead = lead_of(row);
+    const int lane = threadIdx.x & 31, lead = lead_of(row), at = c0 - lead;
     Cut c;
     c.x.x = __shfl_up_sync(0xffffffffu, v.x, 1);
     c.x.y = __shfl_up_sync(0xffffffffu, v.y, 1);
     c.x.z = __shfl_up_sync(0xffffffffu, v.z, 1);
     c.x.w = __shfl_up_sync(0xffffffffu, v.w, 1);
     c.y = v;
-    c.at = 16 - lead * (int)sizeof(T);
-    const bool whole = c0 + N - lead <= dim && (lane > 0 || lead == 0);
-    const bool next = __shfl_down_sync(0xffffffffu, (int)whole, 1) && lane < 31;
-    if (whole) __stcs(reinterpret_cast<uint4*>(row + c0 - lead), lead == 0 ? v : take<false>(c));
-    const int begin = whole ? N - lead : 0, stop = min(next ? N - lead : N, dim - c0);
-    if (begin < stop) store_some(row + c0, v, range_bits(begin, stop));
+    c.at = 16 - lead * (int)sizeof(T);                                // 16: the own block
+    if (at < dim) store_part(row + at, lead == 0 ? v : take<false>(c), lane == 0 ? lead : 0, dim - at);
+    if (lane == 31 && lead > 0 && at + N < dim) {                     // nobody comes behind it
+        c.x = v;
+        store_part(row + at + N, take<false>(c), 0, min(lead, dim - at - N));
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------ lookup
