@@ -521,51 +521,68 @@ template <typename T>
 __device__ __forceinline__ int find_candidates(const Row<T>& row, int top, int shift, float most, TopSpace* t) {
     constexpr int N = Vec<T>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // the bound: a value that `top` of the threads' maxima reach, found bit by bit (the upper 16 bits of the order) by one warp
+    // the bound: a value that `top` of the threads' maxima reach, the upper 16 bits of its order found by one warp, two at a
+    // time (three counts of at most 128 fit into one sum)
     t->most[threadIdx.x] = row.v0 + warp * kBatch + lane < row.v1 ? order_key(most) : 0u;
     if (threadIdx.x == 0) t->n_candidates = 0;
     __syncthreads();
     if (warp == 0) {
+        static_assert(kThreads < 256, "a count has 8 bits");
         uint32_t key[kWarps], bound = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) key[w] = t->most[w * 32 + lane];
 #pragma unroll
-        for (int bit = 31; bit >= 16; --bit) {
-            const uint32_t next = bound | (1u << bit);
-            int n = 0;
+        for (int bit = 30; bit >= 16; bit -= 2) {
+            uint32_t n = 0;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) n += key[w] >= next;
-            if (__reduce_add_sync(0xffffffffu, n) >= top) bound = next;
+            for (int q = 1; q <= 3; ++q)
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) n += key[w] >= (bound | (uint32_t)q << bit) ? 1u << (8 * (q - 1)) : 0u;
+            n = __reduce_add_sync(0xffffffffu, n);
+            if ((int)(n & 0xff) >= top) {                            // fewer reach the larger ones
+                const uint32_t q = (int)(n >> 16 & 0xff) >= top ? 3u : (int)(n >> 8 & 0xff) >= top ? 2u : 1u;
+                bound |= q << bit;
+            }
         }
         if (lane == 0) t->floor = bound;
     }
     __syncthreads();
     const uint32_t low = t->floor;
     const float floor = value_of_key(low);
-    auto take = [&](float v, int j) {
-        const int at = atomicAdd(&t->n_candidates, 1);               // their order does not matter: they are ranked
-        if (at < kCandidates) t->candidate[at] = key_of(v, j);
-    };
     int batch = 0;
     for (int i0 = row.v0 + warp * kBatch; i0 < row.v1; i0 += kWarps * kBatch, ++batch) {
         if (t->maxima[warp][batch >> shift] < floor) continue;
+        uint32_t hits = 0;                                           // which of the lane's kUnroll * N values reach the bound
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k) {
             const int i = i0 + k * 32 + lane;
             if (i >= row.v1) continue;
-            const uint4 r[1] = {row.vec(i)};
-            if (Vec<T>::largest(r) < floor) continue;
             float f[N];
-            mgw_unpack<T, N>(r[0], f);
+            mgw_unpack<T, N>(row.vec(i), f);
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (!(f[e] < floor)) take(f[e], row.head + i * N + e);
+            for (int e = 0; e < N; ++e) hits |= f[e] < floor ? 0u : 1u << (k * N + e);
+        }
+        int before = __popc(hits);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += v;
+        }
+        int at = 0;
+        if (lane == 31) at = atomicAdd(&t->n_candidates, before);    // the order does not matter: keys are ranked
+        at = __shfl_sync(0xffffffffu, at, 31) + before - __popc(hits);
+        for (; hits != 0; hits &= hits - 1, ++at) {
+            const int q = __ffs(hits) - 1, j = row.head + (i0 + q / N * 32 + lane) * N + q % N;
+            if (at < kCandidates) t->candidate[at] = key_of(mgw_to_float(row.z[j]), j);
         }
     }
     const int j = row.edge(threadIdx.x);
     if (j >= 0) {
         const float v = mgw_to_float(row.z[j]);
-        if (!(v < floor)) take(v, j);
+        if (!(v < floor)) {
+            const int at = atomicAdd(&t->n_candidates, 1);
+            if (at < kCandidates) t->candidate[at] = key_of(v, j);
+        }
     }
     __syncthreads();
     const int found = t->n_candidates;
