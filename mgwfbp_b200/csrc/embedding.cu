@@ -858,7 +858,7 @@ int launch_fwd(const void* tokens, int wide, long long n, const void* weight, lo
 }
 
 bool bad_sizes(long long n, long long vocab, int dim, int dtype) {
-    return n < 0 || n > 0x7fffffffLL || vocab < 1 || vocab > 0x7ffffffeLL || dim < 1 || dtype < MGW_F32 || dtype > MGW_BF16;
+    return n < 0 || n > 0x7fffffffLL || vocab < 1 || vocab > 0x7ffffffeLL || dim < 1 || dim > (1 << 30) || dtype < MGW_F32 || dtype > MGW_BF16;
 }
 
 }  // namespace

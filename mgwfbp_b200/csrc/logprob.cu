@@ -15,7 +15,7 @@
 //
 // The likeliest tokens come out of the same pass.  Every thread knows the largest of its logits, so a value that K
 // threads reach is a lower bound for the K-th largest; every warp keeps the maximum of each 128 vectors that it read,
-// and only those that reach the bound are looked at again (from L2).  What reaches the bound is ranked by counting.
+// and only those that reach the bound are looked at again (from L2).  What reaches the bound is sorted, 32 keys to a warp.
 #include <cooperative_groups.h>
 #include "api.h"
 #include "dtypes.cuh"
@@ -28,7 +28,7 @@ constexpr int kMaxTop = 32;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;                 // 16-byte vectors of a thread in a batch
-constexpr int kStages = 3;                 // batches of a warp on their way or in use
+constexpr int kStages = 2;                 // batches of a warp: one in use, one on its way
 constexpr int kBatch = 32 * kUnroll;       // vectors that a warp reads at a time
 constexpr int kMaxima = 128;               // maxima that a warp keeps; neighbouring batches share one beyond that
 constexpr int kCandidates = 512;
@@ -484,10 +484,21 @@ __device__ __forceinline__ Key merge_lists(Key a, Key b) {           // both des
     return x;
 }
 
+// The warps' lists become one, in the first warp.
+__device__ __forceinline__ Key join_lists(Key mine, TopSpace* t) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    t->list[warp][lane] = mine;
+    __syncthreads();
+    if (warp == 0)
+        for (int w = 1; w < kWarps; ++w)
+            if (t->list[w][0] != 0) mine = merge_lists(mine, t->list[w][lane]);
+    return mine;
+}
+
 // Many equal or rising values: every warp keeps a sorted list of the 32 largest and goes through its part of the row, 32
-// values at a time.  The `top` largest keys end up in t->candidate.
+// values at a time.
 template <typename T>
-__device__ __noinline__ int top_by_lists(const Row<T>& row, int top, float floor, TopSpace* t) {
+__device__ __noinline__ Key top_by_lists(const Row<T>& row, float floor, TopSpace* t) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Key mine = 0;
     auto offer = [&](Key x) {
@@ -506,19 +517,13 @@ __device__ __noinline__ int top_by_lists(const Row<T>& row, int top, float floor
         const int j = row.edge(lane);
         offer(j >= 0 ? key_of(mgw_to_float(row.z[j]), j) : (Key)0);
     }
-    t->list[warp][lane] = mine;
-    __syncthreads();
-    if (warp == 0) {
-        for (int w = 1; w < kWarps; ++w) mine = merge_lists(mine, t->list[w][lane]);
-        if (lane < top) t->candidate[lane] = mine;
-    }
-    __syncthreads();
-    return top;
+    return join_lists(mine, t);
 }
 
-// Keys that hold the `top` largest of this block's part of the row: t->candidate[0 .. returned).
+// The 32 largest keys of this block's part of the row (at least the `top` largest are right), in the lanes of the first
+// warp, the largest first.
 template <typename T>
-__device__ __forceinline__ int find_candidates(const Row<T>& row, int top, int shift, float most, TopSpace* t) {
+__device__ __forceinline__ Key find_top(const Row<T>& row, int top, int shift, float most, TopSpace* t) {
     constexpr int N = Vec<T>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // the bound: a value that `top` of the threads' maxima reach, the upper 16 bits of its order found by one warp, two at a
@@ -569,7 +574,7 @@ __device__ __forceinline__ int find_candidates(const Row<T>& row, int top, int s
             if (lane >= o) before += v;
         }
         int at = 0;
-        if (lane == 31) at = atomicAdd(&t->n_candidates, before);    // the order does not matter: keys are ranked
+        if (lane == 31) at = atomicAdd(&t->n_candidates, before);    // the order does not matter: keys are sorted
         at = __shfl_sync(0xffffffffu, at, 31) + before - __popc(hits);
         for (; hits != 0; hits &= hits - 1, ++at) {
             const int q = __ffs(hits) - 1, j = row.head + (i0 + q / N * 32 + lane) * N + q % N;
@@ -586,14 +591,13 @@ __device__ __forceinline__ int find_candidates(const Row<T>& row, int top, int s
     }
     __syncthreads();
     const int found = t->n_candidates;
-    return found <= kCandidates ? found : top_by_lists(row, top, floor, t);
-}
-
-// How many of n keys are larger.
-__device__ __forceinline__ int rank_of(Key x, const Key* keys, int n) {
-    int r = 0;
-    for (int i = 0; i < n; ++i) r += keys[i] > x;
-    return r;
+    if (found > kCandidates) return top_by_lists(row, floor, t);
+    Key mine = 0;
+    for (int at = warp * 32; at < found; at += kThreads) {
+        const Key x = sort_lanes(at + lane < found ? t->candidate[at + lane] : (Key)0);
+        mine = at == warp * 32 ? x : merge_lists(mine, x);
+    }
+    return found <= 32 ? mine : join_lists(mine, t);
 }
 
 // ------------------------------------------------------------------------------------------- gradient of one row
@@ -714,31 +718,20 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
             if (a.stats) a.stats[r] = make_float2(fine ? x.m : mgw_nan(), log2_s);
         }
         if (TOP) {
-            int n = find_candidates(row, a.top, shift, most, top);
-            const Key* from = top->candidate;
-            if (a.splits > 1) {                                      // every block's `top` largest, then those of all
+            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+            Key mine = find_top(row, a.top, shift, most, top);
+            if (a.splits > 1) {
                 cg::cluster_group cluster = cg::this_cluster();
-                if (threadIdx.x < kMaxTop) block_list[threadIdx.x] = 0;
-                __syncthreads();
-                for (int i = threadIdx.x; i < n; i += kThreads) {
-                    const int k = rank_of(from[i], from, n);
-                    if (k < a.top) block_list[k] = from[i];
-                }
+                if (warp == 0) block_list[lane] = mine;
                 cluster.sync();
-                n = a.splits * a.top;
-                if (part == 0)
-                    for (int i = threadIdx.x; i < n; i += kThreads) top->candidate[i] = *cluster.map_shared_rank(&block_list[i % a.top], i / a.top);
-                __syncthreads();
+                if (part == 0 && warp == 0)
+                    for (int k = 1; k < a.splits; ++k) mine = merge_lists(mine, *cluster.map_shared_rank(&block_list[lane], k));
             }
-            if (part == 0)
-                for (int i = threadIdx.x; i < n; i += kThreads) {
-                    const Key key = from[i];
-                    const int k = key != 0 ? rank_of(key, from, n) : a.top;
-                    if (k >= a.top) continue;
-                    const int j = (int)(0xffffffffu - (uint32_t)key);
-                    a.top_tokens[r * a.top + k] = j;
-                    a.top_logprob[r * a.top + k] = fine ? ln_prob<T>(mgw_to_float(row.z[j]), x.m, log2_s) : mgw_nan();
-                }
+            if (part == 0 && warp == 0 && lane < a.top) {
+                const int j = (int)(0xffffffffu - (uint32_t)mine);
+                a.top_tokens[r * a.top + lane] = j;
+                a.top_logprob[r * a.top + lane] = fine ? ln_prob<T>(mgw_to_float(row.z[j]), x.m, log2_s) : mgw_nan();
+            }
         }
         if (LOSS) mgw_wait_for_previous();                               // the count of rows
         if (LOSS && a.dz != nullptr) {                               // the row was just read: it comes from L2
@@ -863,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_bwd_kernel(GradArgs a) {
 
 bool bad_rows(const void* z, long long ld, long long rows, int vocab, int dtype, const void* tokens) {
     const int es = dtype == MGW_F32 ? 4 : 2;
-    return rows < 0 || rows > 0x7fffffffLL || vocab < 1 || (rows > 1 && ld < vocab) || dtype < MGW_F32 || dtype > MGW_BF16 ||
+    return rows < 0 || rows > 0x7fffffffLL || vocab < 1 || vocab > (1 << 30) || (rows > 1 && ld < vocab) || dtype < MGW_F32 || dtype > MGW_BF16 ||
            (rows > 0 && (z == nullptr || tokens == nullptr || ((uintptr_t)z & (es - 1))));
 }
 

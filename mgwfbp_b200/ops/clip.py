@@ -102,6 +102,9 @@ def _launch(grads: List[torch.Tensor], codes: bytes, code: int, scale: float, ma
         if rc == 2:
             raise ValueError('grad_clip: %s' % lib.mgw_last_error().decode(errors='replace'))
         _lib.check(rc, 'grad_clip')
+        if clip:
+            for g in [g for g in grads if g.requires_grad]:        # part of a graph (create_graph): it has changed in place
+                torch.autograd.graph.increment_version(g)
         counters.bump('grad_norm', (n + 1023) // 1024)
         counters.bump('grad_scale' if clip else 'grad_norm_finish', (n + 1023) // 1024 if clip else 1)
     return out

@@ -50,8 +50,12 @@ def _check(tokens: torch.Tensor, weight: torch.Tensor) -> None:
     if weight.is_cuda:
         if weight.dtype not in DTYPE_CODES:
             raise TypeError('weight must be float32, float16 or bfloat16, got %s' % weight.dtype)
-        if weight.shape[0] > 0x7ffffffe or tokens.numel() > 0x7fffffff:
-            raise ValueError('more than 2^31 - 2 rows or 2^31 - 1 tokens')
+        _check_sizes(tokens.numel(), *weight.shape)
+
+
+def _check_sizes(n: int, vocab: int, dim: int) -> None:
+    if n > 0x7fffffff or vocab > 0x7ffffffe or dim > 1 << 30:
+        raise ValueError('more than 2^31 - 1 tokens, 2^31 - 2 rows or 2^30 columns')
 
 
 def _padding(padding_idx: Optional[int], vocab: int) -> int:
@@ -102,8 +106,7 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, num_embeddings: int
         return (dw * scale).to(grad.dtype)
     if grad.dtype not in DTYPE_CODES:
         raise TypeError('grad must be float32, float16 or bfloat16, got %s' % grad.dtype)
-    if num_embeddings > 0x7ffffffe or n > 0x7fffffff:
-        raise ValueError('more than 2^31 - 2 rows or 2^31 - 1 tokens')
+    _check_sizes(n, num_embeddings, dim)
     return _grad_cuda(grad, tokens, num_embeddings, scale, padding)
 
 
@@ -165,7 +168,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
 
 class FusedEmbedding(nn.Embedding):
     """``nn.Embedding`` (same parameter and ``state_dict`` key) whose lookup and gradient run this package's kernels, with an
-    optional factor on the rows (``scale``).  The options ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are refused."""
+    optional factor on the rows (``scale``).  A table of a type that the kernels do not have (float64) runs the parent's
+    lookup.  The options ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are refused."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None, scale: float = 1.0, **kwargs):
         for option in ('max_norm', 'scale_grad_by_freq', 'sparse'):
@@ -175,6 +179,8 @@ class FusedEmbedding(nn.Embedding):
         self.scale = float(scale)
 
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+        if self.weight.is_cuda and self.weight.dtype not in DTYPE_CODES:
+            return super().forward(tokens) * self.scale
         return embedding(tokens, self.weight, self.scale, self.padding_idx)
 
     def extra_repr(self) -> str:

@@ -67,8 +67,8 @@ def _check(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> None:
     if logits.is_cuda:
         if logits.dtype not in DTYPE_CODES:
             raise TypeError('logits must be float32, float16 or bfloat16, got %s' % logits.dtype)
-        if tokens.numel() > 0x7fffffff or logits.shape[-1] > 0x7fffffff:
-            raise ValueError('more than 2^31 - 1 rows or columns')
+        if tokens.numel() > 0x7fffffff or logits.shape[-1] > 1 << 30:
+            raise ValueError('more than 2^31 - 1 rows or 2^30 columns')
     elif not logits.is_floating_point():
         raise TypeError('logits must be floating point, got %s' % logits.dtype)
 
@@ -257,7 +257,8 @@ def cross_entropy(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int 
 
 class FusedCrossEntropyLoss(nn.CrossEntropyLoss):
     """``nn.CrossEntropyLoss`` over class indices that runs this package's kernels: logits ``[rows, vocabulary]`` (or one
-    row), no class weights, no label smoothing.  ``expected_grad``: see :func:`cross_entropy`."""
+    row), no class weights, no label smoothing.  Logits of a type that the kernels do not have (float64) run the parent's
+    loss.  ``expected_grad``: see :func:`cross_entropy`."""
 
     def __init__(self, ignore_index: int = -100, reduction: str = 'mean', expected_grad: float = 1.0):
         super().__init__(ignore_index=ignore_index, reduction=reduction)
@@ -266,4 +267,6 @@ class FusedCrossEntropyLoss(nn.CrossEntropyLoss):
     def forward(self, logits: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
         if logits.dim() > 2:
             raise ValueError('FusedCrossEntropyLoss takes [rows, vocabulary] logits, got shape %s' % (tuple(logits.shape),))
+        if logits.is_cuda and logits.dtype not in DTYPE_CODES:
+            return super().forward(logits, tokens)
         return cross_entropy(logits, tokens, self.ignore_index, self.reduction, self.expected_grad)

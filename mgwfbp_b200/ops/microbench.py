@@ -7,6 +7,9 @@ measured roofline (``MEASURED_PEAKS.json`` at the repository root when present).
     python -m mgwfbp_b200.ops.microbench wgrad --k 64 --m 4096 --n 25088 [--sgd]
     python -m mgwfbp_b200.ops.microbench pack  --numel 25557032          # fused all-reduce kernel, world size 1
     python -m mgwfbp_b200.ops.microbench fused                            # all of ResNet-50 as one group: all-reduce + SGD
+    python -m mgwfbp_b200.ops.microbench embedding --rows 700 --vocab 10000 --channels 1500 [--dtype bf16]
+    python -m mgwfbp_b200.ops.microbench logprob   --rows 700 --vocab 10000 --top 5 [--dtype bf16]    # and the mean loss
+    python -m mgwfbp_b200.ops.microbench clip      --numel 66034000 [--dtype bf16]
 
 Timing: CUDA events on the launching stream, ``--warmup`` untimed launches, a write larger than L2
 between timed launches, median of ``--iters``; the last line printed is the SM clock / throttle-reason
@@ -177,9 +180,48 @@ def bench_fused(args, timer):
     comm.check_status(synchronize=True)
 
 
+_DTYPES = {'fp32': torch.float32, 'fp16': torch.float16, 'bf16': torch.bfloat16}
+
+
+def bench_embedding(args, timer):
+    from .embedding import check_status, embedding, embedding_grad
+    n, vocab, dim, dt = args.rows, args.vocab, args.channels, _DTYPES[args.dtype]
+    size = torch.finfo(dt).bits // 8
+    w = torch.randn(vocab, dim, device='cuda').to(dt)
+    t = torch.randint(0, vocab, (n,), device='cuda')
+    dy = torch.randn(n, dim, device='cuda').to(dt)
+    name = '%s, %d of %d x %d' % (args.dtype, n, vocab, dim)
+    report('embedding_fwd[%s]' % name, timer(lambda: embedding(t, w)), nbytes=size * dim * (n + min(n, vocab)) + 8 * n)
+    report('embedding_grad[%s]' % name, timer(lambda: embedding_grad(dy, t, vocab)), nbytes=size * dim * (n + vocab) + 8 * n)
+    check_status()
+
+
+def bench_logprob(args, timer):
+    from .logprob import cross_entropy, token_log_probs
+    n, vocab, dt = args.rows, args.vocab, _DTYPES[args.dtype]
+    size = torch.finfo(dt).bits // 8
+    z = torch.randn(n, vocab, device='cuda').to(dt)
+    t = torch.randint(0, vocab, (n,), device='cuda')
+    name = '%s, %d x %d' % (args.dtype, n, vocab)
+    report('token_log_probs[%s, top %d]' % (name, args.top), timer(lambda: token_log_probs(z, t, top=args.top)), nbytes=size * n * vocab)
+    zg = z.clone().requires_grad_()
+    report('cross_entropy with gradient[%s]' % name, timer(lambda: cross_entropy(zg, t)), nbytes=2 * size * n * vocab)
+
+
+def bench_clip(args, timer):
+    from .clip import clip_grad_norm_, grad_norm
+    dt = _DTYPES[args.dtype]
+    size = torch.finfo(dt).bits // 8
+    p = torch.nn.Parameter(torch.empty(args.numel, device='cuda', dtype=dt))
+    p.grad = torch.randn(args.numel, device='cuda').to(dt)
+    name = '%s, %d elements' % (args.dtype, args.numel)
+    report('grad_norm[%s]' % name, timer(lambda: grad_norm([p.grad])), nbytes=size * args.numel)
+    report('clip_grad_norm_[%s]' % name, timer(lambda: clip_grad_norm_(p, 0.25, grad_scale=2.0)), nbytes=3 * size * args.numel)
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument('what', choices=['bn', 'sgd', 'wgrad', 'pack', 'fused'])
+    ap.add_argument('what', choices=['bn', 'sgd', 'wgrad', 'pack', 'fused', 'embedding', 'logprob', 'clip'])
     ap.add_argument('--rows', type=int, default=200704)
     ap.add_argument('--channels', type=int, default=256)
     ap.add_argument('--residual', action='store_true')
@@ -188,6 +230,9 @@ def main(argv=None):
     ap.add_argument('--m', type=int, default=4096)
     ap.add_argument('--n', type=int, default=25088)
     ap.add_argument('--sgd', action='store_true')
+    ap.add_argument('--vocab', type=int, default=10000)
+    ap.add_argument('--top', type=int, default=5)
+    ap.add_argument('--dtype', choices=['fp32', 'fp16', 'bf16'], default='fp32')
     ap.add_argument('--iters', type=int, default=10)
     ap.add_argument('--warmup', type=int, default=3)
     args = ap.parse_args(argv)
@@ -203,7 +248,8 @@ def main(argv=None):
 
 
 def _run(args, timer):
-    {'bn': bench_bn, 'sgd': bench_sgd, 'wgrad': bench_wgrad, 'pack': bench_pack, 'fused': bench_fused}[args.what](args, timer)
+    {'bn': bench_bn, 'sgd': bench_sgd, 'wgrad': bench_wgrad, 'pack': bench_pack, 'fused': bench_fused,
+     'embedding': bench_embedding, 'logprob': bench_logprob, 'clip': bench_clip}[args.what](args, timer)
 
 
 if __name__ == '__main__':

@@ -52,6 +52,45 @@ def test_embedding_forward_and_gradient(n, vocab, dim, kind, dtype):
     check_status()
 
 
+@pytest.mark.parametrize('dtype', TYPES, ids=ids)
+def test_embedding_every_width_and_alignment(dtype):
+    """Rows that begin and end anywhere in a 16-byte block, in the table, the output, the gradient and its sum; short lists
+    (one launch), longer ones, and ones that leave most rows without a token."""
+    from mgwfbp_b200.ops.embedding import embedding, embedding_grad
+    gen = torch.Generator(device='cuda').manual_seed(7)
+    store = torch.randn(4, 41, 600, device='cuda', generator=gen).to(dtype)
+    for dim in list(range(1, 41)) + [63, 64, 65, 127, 128, 129, 255, 256, 257, 258, 383, 511, 512, 513, 590]:
+        for at in range(0, 8 if dim < 41 else 3):
+            w = store[dim % 4, :, at:at + dim]                       # rows 600 apart, from any element
+            for n in (5, 1500):
+                t = torch.randint(0, 41, (n,), device='cuda', generator=gen)
+                assert torch.equal(embedding(t, w), w[t]), (dim, at, n)
+                wide = torch.randn(n, dim + at + 3, device='cuda', generator=gen).to(dtype)
+                dy = wide[:, at:at + dim]
+                want, bound = oracle_grad(dy, t, 43, 1.0)
+                assert_within(embedding_grad(dy, t, 43), want, bound, 'dw %d %d %d' % (dim, at, n))
+
+
+def test_embedding_gradient_writes_nothing_else():
+    """The rows behind and before the result stay as they were."""
+    from mgwfbp_b200.ops import embedding as emb
+    lib = emb._lib_ready()
+    for n in (6, 3000, 70000):
+        for dim, shift in ((37, 3), (64, 0)):
+            t = torch.randint(0, 50, (n,), device='cuda')
+            dy = torch.randn(n, dim, device='cuda')
+            store = torch.full((60 * dim + 16,), 7.0, device='cuda')
+            dw = store[5 * dim + shift:55 * dim + shift]
+            need = lib.mgw_embedding_grad_bytes(n, 50, dim, 0)
+            work = torch.empty(need, dtype=torch.uint8, device='cuda')
+            assert lib.mgw_embedding_grad(dy.data_ptr(), dim, t.data_ptr(), 1, n, 50, dim, 0, 1.0, -1, dw.data_ptr(),
+                                          work.data_ptr() if need else None, need, emb.status_words(),
+                                          torch.cuda.current_stream().cuda_stream) == 0
+            want, bound = oracle_grad(dy, t, 50, 1.0)
+            assert_within(dw.view(50, dim), want, bound, 'dw')
+            assert (store[:5 * dim + shift] == 7).all() and (store[55 * dim + shift:] == 7).all()
+
+
 def test_embedding_strides_shapes_and_broadcast_gradient():
     from mgwfbp_b200.ops.embedding import embedding, embedding_grad
     wide = torch.randn(50, 40, device='cuda')
@@ -260,6 +299,50 @@ def test_gradients_against_differences():
                                                       (Rows(z.detach().double() + s * v, t).entropy()[0], 0.5)))
     got, want = float((dz.double() * v).sum()), (f(1e-5) - f(-1e-5)) / 2e-5
     assert abs(got - want) <= 1e-4 * max(1.0, float((dz.double() * v).abs().sum()))
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=ids)
+def test_log_probs_every_width_and_alignment(dtype):
+    """Vocabularies around the sizes of a vector, a batch, a block and a cluster's parts, rows that begin anywhere."""
+    from mgwfbp_b200.ops.logprob import cross_entropy, token_log_probs
+    gen = torch.Generator(device='cuda').manual_seed(9)
+    widths = list(range(1, 36)) + [k + d for k in (128, 512, 1024, 2048, 4096, 8192, 16384) for d in (-1, 0, 1, 5)]
+    for v in widths:
+        for rows, at in ((3, v % 8), (2, (v + 3) % 8)):
+            wide = (torch.randn(rows, v + 9, device='cuda', generator=gen) * 3).to(dtype)
+            z = wide[:, at:at + v].detach().requires_grad_()
+            t = torch.randint(0, v, (rows,), device='cuda', generator=gen)
+            top = min(7, v)
+            want = Rows(z, t)
+            r = token_log_probs(z, t, top=top)
+            assert_within(r.logprob, *want.logprob(), 'logprob %d' % v)
+            assert_within(r.entropy, *want.entropy(), 'entropy %d' % v)
+            assert torch.equal(r.top_tokens, want.top(top)[2]), v
+            g1, g2 = torch.randn(rows, device='cuda', generator=gen), torch.randn(rows, device='cuda', generator=gen)
+            (dz,) = torch.autograd.grad([r.logprob, r.entropy], [z], [g1, g2])
+            assert_within(dz, *want.grad(g1, g2, dtype), 'dz %d' % v)
+            (dz,) = torch.autograd.grad(cross_entropy(z, t), z)
+            assert_within(dz, *want.grad(-torch.ones(rows, device='cuda') / rows, g2 * 0, dtype), 'dloss %d' % v)
+
+
+@pytest.mark.parametrize('rows', [2, 700])
+def test_top_of_sorted_rows_and_ties(rows):
+    """Rows in rising and falling order, in plateaus, with the largest values in one vector, at the ends, or all equal."""
+    from mgwfbp_b200.ops.logprob import token_log_probs
+    for dtype in TYPES:
+        for v in (50261, 10000, 700):
+            base = torch.linspace(-4, 9, v, device='cuda')
+            kinds = [base, base.flip(0), (base * 3).round() / 3, torch.zeros(v, device='cuda'), base * 0 - 1e4, base.clone()]
+            kinds[4][v - 3:] = 5.0
+            kinds[4][:2] = 5.0
+            kinds[5][v // 2:v // 2 + 24] = 11.0
+            z = torch.stack([kinds[i % len(kinds)] for i in range(rows)]).to(dtype)
+            t = torch.zeros(rows, dtype=torch.int64, device='cuda')
+            for top in (1, 20, 32):
+                r = token_log_probs(z, t, top=top)
+                lp, bound, order = Rows(z, t).top(top)
+                assert torch.equal(r.top_tokens, order)
+                assert_within(r.top_logprob, lp, bound, 'top')
 
 
 def test_log_probs_shapes_and_strides():
@@ -524,6 +607,44 @@ def test_operators_on_another_stream_and_in_two_graphs():
                 assert torch.equal(a, b)
     from mgwfbp_b200.ops.embedding import check_status
     check_status()
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first use of the operators is being captured."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from test_gpu_lm_ops import _together, _together_inputs, _together_net
+net, data = _together_net(), _together_inputs(4)
+a = torch.randn(64, 64, device='cuda', requires_grad=True)
+torch.autograd.grad((a @ a).sum(), a)                      # the library's own first calls
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = _together(net, *data)
+g.replay()
+torch.cuda.synchronize()
+got = [v.clone() for v in got]
+want = _together(net, *data)
+assert all(torch.equal(x, y) for x, y in zip(got, want))
+print('captured')
+"""
+    import os
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(here)]))
+    out = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, timeout=300, env=env)
+    assert out.returncode == 0 and 'captured' in out.stdout, out.stderr[-2000:]
+
+
+def test_other_types_run_the_parents():
+    from mgwfbp_b200.ops.embedding import FusedEmbedding
+    from mgwfbp_b200.ops.logprob import FusedCrossEntropyLoss
+    t = torch.tensor([1, 3], device='cuda')
+    e = FusedEmbedding(5, 4, scale=2.0).cuda().double()
+    assert torch.equal(e(t), e.weight[t] * 2.0)
+    z = torch.randn(2, 5, device='cuda', dtype=torch.float64)
+    assert torch.equal(FusedCrossEntropyLoss()(z, t), torch.nn.functional.cross_entropy(z, t))
 
 
 def test_native_launches_are_counted():
