@@ -3,10 +3,15 @@
 //   out[i, :] = scale * W[t_i, :]                      dW[v, :] = scale * sum over i with t_i = v of dy[i, :]
 //
 // The gradient's sums are taken in fp32 in the order of the positions i, so the result does not depend on how blocks
-// are scheduled: the tokens are sorted (stable), the sorted list is cut into chunks of equal length -- however often
-// a single word occurs -- and a warp adds up the rows of one chunk for 32 vectors of columns.  A run of equal tokens
-// that lies inside a chunk is stored at once; a run that crosses a border leaves fp32 partial sums, which a second kernel
-// adds up in the order of the chunks.  Rows that no token names are filled with zeros by the same launch.
+// are scheduled, and rounded once: the tokens are sorted (stable), the sorted list is cut into chunks of equal length --
+// however often a single word occurs -- and a warp adds up the rows of one chunk for 512 bytes of columns.  A run of equal
+// tokens inside a chunk is stored at once.  A run that crosses the borders of chunks is put together in the order of the
+// chunks, in shared memory within a block and through fp32 partial sums and a second launch between blocks.  Rows that no
+// token names are filled with zeros by other blocks of the same launch, beside the sort where they can.
+//
+// Everything here is bound by memory once the lists are long: 262,144 rows of 2048 bf16 values of a table of 131,072 take
+// 221 us to look up (1.3 GB, 6.0 TB/s) and 305 us to add up (1.6 GB, 5.3 TB/s; of it 40 us are the sort, which has nothing
+// to hide behind).  700 rows of 1500 fp32 values of a table of 10,000: 2.7 + 14 us, the latter 64 MB of which 60 MB are zeros.
 #include <cooperative_groups.h>
 #include <atomic>
 #include <mutex>
@@ -34,15 +39,24 @@ int launch_dependent(void (*kernel)(P...), long long grid, int threads, size_t s
     return MGW_OK;
 }
 
+// A tile of the radix sort: 2048 entries by 512 threads (by 256 threads with 8 each a pass of 262,144 entries took 15 us
+// instead of 9).
 constexpr int kSortThreads = 512;
 constexpr int kSortItems = 4;
 constexpr int kSortTile = kSortThreads * kSortItems;
 constexpr int kMaxDigitBits = 10;
 
 // --------------------------------------------------------------------------------------------------- blocks of a row
-// Rows move in blocks of 16 bytes.  EXACT: all rows of both matrices begin on 16-byte boundaries and consist of whole
-// blocks.  Otherwise every row is aligned differently: a block is cut out of two aligned vectors when it is read, and put
-// together from two lanes' values when it is stored.
+// How a warp moves 512 bytes of a row, 16 for each lane:
+//   kExact  all rows of both matrices begin on 16-byte boundaries and consist of whole blocks of 16 bytes, one per lane;
+//   kWords  rows begin and end on 4-byte boundaries: a lane has four words, 32 words apart, which moves whole lines as well
+//           and needs no shifting.  200,000 rows of 1023 fp32 values: gradient 210 us, lookup 165 us (rows of 1024, kExact:
+//           199 and 155 us; the rows of 1023 by kShift: 259 and 214 us);
+//   kShift  anything else (16-bit types, odd widths): blocks are cut out of two aligned vectors when they are read, and put
+//           together from two lanes' values when they are stored.  20,011 rows of 1023 fp16 values: lookup 17 us, 23 us with
+//           single 16-bit accesses (rows of 1024: 11 us).
+enum { kExact = 0, kWords = 1, kShift = 2 };
+
 template <typename T> constexpr int per_block() { return 16 / (int)sizeof(T); }
 
 // Elements between the last 16-byte boundary and the row.
@@ -57,14 +71,30 @@ __device__ __forceinline__ bool inside(const T* row, int dim, const char* lo, co
     return reinterpret_cast<const char*>(row) - 31 >= lo && reinterpret_cast<const char*>(row + dim) + 32 <= hi;
 }
 
-// The columns [c0, c0 + N); c0 may be up to N - 1 below the row's first column, or in its last block.
-template <typename T, bool EXACT>
-__device__ __forceinline__ Cut load_block(const T* row, int c0) {
-    const char* s = reinterpret_cast<const char*>(row + c0);
+// Elements from one word of a lane to its next, and the first column of a lane in the row's 512-byte part `part`.
+template <typename T> constexpr int word_step() { return 128 / (int)sizeof(T); }
+template <typename T, int MODE>
+__device__ __forceinline__ int column_of(int part, int lane) {
+    return part * 32 * per_block<T>() + lane * (MODE == kWords ? 4 / (int)sizeof(T) : per_block<T>());
+}
+
+// A lane's values from column c0 on.  kShift: c0 may be up to N - 1 below the row's first column, or in its last block.
+template <typename T, int MODE>
+__device__ __forceinline__ Cut load_block(const T* row, int c0, int dim) {
     Cut r;
-    r.at = EXACT ? 0 : (int)((unsigned long long)s & 15);
+    r.at = 0;
+    const char* s = reinterpret_cast<const char*>(row + c0);
+    if (MODE == kWords) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(s);
+        r.x.x = c0 < dim ? w[0] : 0u;
+        r.x.y = c0 + word_step<T>() < dim ? w[32] : 0u;
+        r.x.z = c0 + 2 * word_step<T>() < dim ? w[64] : 0u;
+        r.x.w = c0 + 3 * word_step<T>() < dim ? w[96] : 0u;
+        return r;
+    }
+    if (MODE == kShift) r.at = (int)((unsigned long long)s & 15);
     r.x = *reinterpret_cast<const uint4*>(s - r.at);
-    if (!EXACT) r.y = *reinterpret_cast<const uint4*>(s - r.at + 16);
+    if (MODE == kShift) r.y = *reinterpret_cast<const uint4*>(s - r.at + 16);
     return r;
 }
 
@@ -81,9 +111,9 @@ __device__ __noinline__ uint4 gather_block(const T* row, int c0, int dim) {
 
 // The block that a Cut holds.  (Selects instead of a branch for each offset: these kernels are large enough that a copy
 // of their inner loop for each offset costs more in instruction fetches than it saves.)
-template <bool EXACT>
+template <int MODE>
 __device__ __forceinline__ uint4 take(const Cut& c) {
-    if (EXACT) return c.x;
+    if (MODE != kShift) return c.x;
     const uint32_t bits = (c.at & 3) * 8;
     const bool two = c.at & 8, one = c.at & 4;
     const uint32_t a0 = two ? c.x.z : c.x.x, a1 = two ? c.x.w : c.x.y, a2 = two ? c.y.x : c.x.z, a3 = two ? c.y.y : c.x.w,
@@ -93,20 +123,8 @@ __device__ __forceinline__ uint4 take(const Cut& c) {
                       __funnelshift_r(b3, b4, bits));
 }
 
-// The elements [begin, stop) of a block at a 16-byte boundary: one store for a whole block, else up to three towards the
+// The elements [begin, stop) of a block (of a 16-bit type) at a 16-byte boundary: one store for a whole block, else up to three towards the
 // middle and three behind it, each as wide as its place allows.
-__device__ __forceinline__ void store_part(float* at, const uint4& v, int begin, int stop) {
-    if (begin <= 0 && stop >= 4) {
-        __stcs(reinterpret_cast<uint4*>(at), v);
-        return;
-    }
-    uint32_t* w = reinterpret_cast<uint32_t*>(at);
-    if (begin <= 0 && 0 < stop) w[0] = v.x;
-    if (begin <= 1 && 1 < stop) w[1] = v.y;
-    if (begin <= 2 && 2 < stop) w[2] = v.z;
-    if (begin <= 3 && 3 < stop) w[3] = v.w;
-}
-
 template <typename T>
 __device__ __forceinline__ void store_part(T* at, const uint4& v, int begin, int stop) {
     if (begin <= 0 && stop >= 8) {
@@ -125,47 +143,57 @@ __device__ __forceinline__ void store_part(T* at, const uint4& v, int begin, int
     if (e < stop) *reinterpret_cast<uint16_t*>(p + 2 * e) = (uint16_t)word(e);
 }
 
-// A block that begins on a boundary, or the part of it in [0, dim).
-template <typename T, bool EXACT>
+template <typename T>
+__device__ __forceinline__ void store_words(T* row, int c0, int dim, const uint4& v) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(row + c0);
+    if (c0 < dim) __stcs(w, v.x);
+    if (c0 + word_step<T>() < dim) __stcs(w + 32, v.y);
+    if (c0 + 2 * word_step<T>() < dim) __stcs(w + 64, v.z);
+    if (c0 + 3 * word_step<T>() < dim) __stcs(w + 96, v.w);
+}
+
+// A lane's values from column c0 on; kShift: the part in [0, dim) of a block that begins on a boundary.
+template <typename T, int MODE>
 __device__ __forceinline__ void store_block(T* row, int c0, int dim, const uint4& v) {
-    if (EXACT) __stcs(reinterpret_cast<uint4*>(row + c0), v);
+    if constexpr (MODE == kExact) __stcs(reinterpret_cast<uint4*>(row + c0), v);
+    else if constexpr (MODE == kWords) store_words(row, c0, dim, v);
     else store_part(row + c0, v, -c0, dim - c0);
 }
 
-// A warp's 32 neighbouring blocks, lane's at column c0 (all lanes take part; those with c0 >= dim have nothing).  With the
-// row `lead` elements behind a boundary, a lane stores the block that begins `lead` before its own: the last elements of
+// A warp's part of a row, the lane's values from column c0 on (all lanes take part; those with c0 >= dim have nothing).
+// kShift: with the row `lead` elements behind a boundary, a lane stores the block that begins `lead` before its own: the last elements of
 // the lane before it and its own first ones.
-template <typename T, bool EXACT>
+template <typename T, int MODE>
 __device__ __forceinline__ void store_blocks(T* row, int c0, int dim, const uint4& v) {
-    constexpr int N = per_block<T>();
-    if (EXACT) {
-        if (c0 < dim) __stcs(reinterpret_cast<uint4*>(row + c0), v);
-        return;
-    }
-    const int lane = threadIdx.x & 31, lead = lead_of(row), at = c0 - lead;
-    Cut c;
-    c.x.x = __shfl_up_sync(0xffffffffu, v.x, 1);
-    c.x.y = __shfl_up_sync(0xffffffffu, v.y, 1);
-    c.x.z = __shfl_up_sync(0xffffffffu, v.z, 1);
-    c.x.w = __shfl_up_sync(0xffffffffu, v.w, 1);
-    c.y = v;
-    c.at = 16 - lead * (int)sizeof(T);                                // 16: the own block
-    if (at < dim) store_part(row + at, lead == 0 ? v : take<false>(c), lane == 0 ? lead : 0, dim - at);
-    if (lane == 31 && lead > 0 && at + N < dim) {                     // nobody comes behind it
-        c.x = v;
-        store_part(row + at + N, take<false>(c), 0, min(lead, dim - at - N));
+    if constexpr (MODE != kShift) {
+        if (c0 < dim) store_block<T, MODE>(row, c0, dim, v);
+    } else {
+        constexpr int N = per_block<T>();
+        const int lane = threadIdx.x & 31, lead = lead_of(row), at = c0 - lead;
+        Cut c;
+        c.x.x = __shfl_up_sync(0xffffffffu, v.x, 1);
+        c.x.y = __shfl_up_sync(0xffffffffu, v.y, 1);
+        c.x.z = __shfl_up_sync(0xffffffffu, v.z, 1);
+        c.x.w = __shfl_up_sync(0xffffffffu, v.w, 1);
+        c.y = v;
+        c.at = 16 - lead * (int)sizeof(T);                            // 16: the own block
+        if (at < dim) store_part(row + at, lead == 0 ? v : take<kShift>(c), lane == 0 ? lead : 0, dim - at);
+        if (lane == 31 && lead > 0 && at + N < dim) {                 // nobody comes behind it
+            c.x = v;
+            store_part(row + at + N, take<kShift>(c), 0, min(lead, dim - at - N));
+        }
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------ lookup
 // Blocks that a lane keeps in flight; one more for rows between boundaries, which may have a block more than their length.
-constexpr int lookup_unroll(bool exact) { return exact ? 4 : 5; }
+constexpr int lookup_unroll(int mode) { return mode == kShift ? 5 : 4; }
 
-template <typename T, bool EXACT>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(256, 3)
 embedding_fwd_kernel(const void* __restrict__ tokens, int wide, long long n, const T* __restrict__ weight, long long ld,
                      long long vocab, int dim, float scale, T* __restrict__ out, int segments, int* status) {
-    constexpr int N = per_block<T>(), U = lookup_unroll(EXACT);
+    constexpr int N = per_block<T>(), U = lookup_unroll(MODE);
     const int lane = threadIdx.x & 31;
     const long long warps = (long long)gridDim.x * (blockDim.x >> 5);
     const char* lo = reinterpret_cast<const char*>(weight);
@@ -186,17 +214,17 @@ embedding_fwd_kernel(const void* __restrict__ tokens, int wide, long long n, con
                 for (int e = 0; e < N; ++e) f[e] = valid ? f[e] * scale : mgw_nan();
                 v = mgw_pack<T, N>(f);
             }
-            store_block<T, EXACT>(dst, c, dim, v);
+            store_block<T, MODE>(dst, c, dim, v);
         };
-        const int c = (seg * 32 * U + lane) * N - (EXACT ? 0 : lead_of(dst));
-        if (EXACT || inside(src, dim, lo, hi)) {
+        const int c = column_of<T, MODE>(seg * U, lane) - (MODE == kShift ? lead_of(dst) : 0);
+        if (MODE != kShift || inside(src, dim, lo, hi)) {
             Cut r[U];
 #pragma unroll
             for (int k = 0; k < U; ++k)
-                if (c + 32 * N * k < dim) r[k] = load_block<T, EXACT>(src, c + 32 * N * k);
+                if (c + 32 * N * k < dim) r[k] = load_block<T, MODE>(src, c + 32 * N * k, dim);
 #pragma unroll
             for (int k = 0; k < U; ++k)
-                if (c + 32 * N * k < dim) put(take<EXACT>(r[k]), c + 32 * N * k);
+                if (c + 32 * N * k < dim) put(take<MODE>(r[k]), c + 32 * N * k);
         } else {
 #pragma unroll 1
             for (int k = 0; k < U; ++k)
@@ -343,9 +371,10 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) 
     }
 }
 
-// Short lists: the whole sort in one launch of one cluster, which keeps the list in its shared memory.  A block has a
-// contiguous part of it; per pass the blocks read each other's histograms and write every entry to its new place, which may
-// be another block's memory.
+// Lists of up to 65,536 tokens: the whole sort in one launch of one cluster, which keeps the list in its shared memory.  A
+// block has a contiguous part of it; per pass the blocks read each other's histograms and write every entry to its new place,
+// which may be another block's memory.  10 us up to 8192 tokens, 18 us for 32,768, 30 us for 65,536, where the six launches
+// of the tiled sort are as fast.
 constexpr int kCluster = 8;
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterItems = 8;
@@ -447,7 +476,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThrea
 
 // The same within one block of 1024 threads, for at most 1024 tokens, one per thread; the sorted list is left in shared memory.
 constexpr int kSmallWarps = 32;
-constexpr int kSmallList = kSmallWarps * 32;                          // up to here one launch does it all
+constexpr int kSmallList = kSmallWarps * 32;                          // up to here one launch does it all: 12.3 instead of 12.6 us
+                                                                      // for 700 tokens (10000 x 512), 14.7 instead of 13.7 for 1024
 
 struct SmallSort {
     uint16_t cnt[kSmallWarps][1 << kClusterBits];
@@ -523,7 +553,7 @@ struct GradArgs {
 constexpr int kZeroRows = 1024;            // most rows of a block that fills
 
 constexpr int kSumWarps = 8;
-constexpr int kMaxChunk = 64;
+constexpr int kMaxChunk = 64;              // 262,144 tokens: 307 us; 314 with 256, 316 with 512 (fewer, less even parts)
 
 // fp32 partial sums of a slab: the values of a lane one behind the other
 template <typename T>
@@ -532,7 +562,7 @@ __device__ __forceinline__ float4* partial_of(const GradArgs& a, long long group
 }
 
 // A block's rows that no token names.
-template <typename T, bool EXACT>
+template <typename T, int MODE>
 __device__ __forceinline__ void fill_rows(const GradArgs& a, long long block) {
     __shared__ uint32_t named[kZeroRows / 32];
     const long long r0 = block * a.zero_rows, r1 = min(a.vocab, r0 + a.zero_rows);
@@ -565,8 +595,8 @@ __device__ __forceinline__ void fill_rows(const GradArgs& a, long long block) {
     for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += blockDim.x >> 5) {
         if (named[(r - r0) >> 5] >> ((r - r0) & 31) & 1) continue;
         T* row = static_cast<T*>(a.dw) + r * a.dim;
-        for (int c = lane * per_block<T>() - (EXACT ? 0 : lead_of(row)); c < a.dim; c += 32 * per_block<T>())
-            store_block<T, EXACT>(row, c, a.dim, zero);
+        for (int c = column_of<T, MODE>(0, lane) - (MODE == kShift ? lead_of(row) : 0); c < a.dim; c += 32 * per_block<T>())
+            store_block<T, MODE>(row, c, a.dim, zero);
     }
 }
 
@@ -578,11 +608,11 @@ struct SumSpace {
 };
 
 // The chunks of a group, one per warp, for the columns of a slab.
-template <typename T, bool EXACT, int WARPS>
+template <typename T, int MODE, int WARPS>
 __device__ __forceinline__ void sum_group(const GradArgs& a, const uint2* list, long long group, int slab, SumSpace<T, WARPS>& m) {
     constexpr int N = per_block<T>(), U = 4;                          // rows in flight
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = (slab * 32 + lane) * N;
-    const int c = min(c0, (a.dim - 1) / N * N);                       // lanes behind the row's end read its last block
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = column_of<T, MODE>(slab, lane);
+    const int c = MODE == kWords ? c0 : min(c0, (a.dim - 1) / N * N); // lanes behind the row's end read its last block
     const T* dy = static_cast<const T*>(a.dy);
     const char* lo = static_cast<const char*>(a.dy);
     const char* hi = reinterpret_cast<const char*>(dy + (a.n - 1) * a.dy_ld + a.dim);
@@ -603,7 +633,7 @@ __device__ __forceinline__ void sum_group(const GradArgs& a, const uint2* list, 
     auto store = [&](uint32_t key) {
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] *= a.scale;
-        store_blocks<T, EXACT>(dw + (long long)key * a.dim, c0, a.dim, mgw_pack<T, N>(acc));
+        store_blocks<T, MODE>(dw + (long long)key * a.dim, c0, a.dim, mgw_pack<T, N>(acc));
     };
     auto flush = [&](bool goes_on) {
         if (comes_in || goes_on) {
@@ -631,21 +661,21 @@ __device__ __forceinline__ void sum_group(const GradArgs& a, const uint2* list, 
         const uint2 mine = b0 + lane < i1 ? list[b0 + lane] : make_uint2(none, 0u);
         const int here = __popc(__ballot_sync(0xffffffffu, mine.x != none));
         // rows at the ends of dy, whose blocks cannot be cut out of vectors
-        const bool edge = !EXACT && lane < here && !inside(dy + (long long)mine.y * a.dy_ld, a.dim, lo, hi);
-        const unsigned edges = EXACT ? 0u : __ballot_sync(0xffffffffu, edge);
+        const bool edge = MODE == kShift && lane < here && !inside(dy + (long long)mine.y * a.dy_ld, a.dim, lo, hi);
+        const unsigned edges = MODE != kShift ? 0u : __ballot_sync(0xffffffffu, edge);
         for (int j = 0; j < here; ) {
             if (j + U <= here && (edges >> j & ((1u << U) - 1u)) == 0) {
                 Cut r[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    r[u] = load_block<T, EXACT>(dy + (long long)__shfl_sync(0xffffffffu, mine.y, j + u) * a.dy_ld, c);
+                    r[u] = load_block<T, MODE>(dy + (long long)__shfl_sync(0xffffffffu, mine.y, j + u) * a.dy_ld, c, a.dim);
 #pragma unroll
-                for (int u = 0; u < U; ++u) add(__shfl_sync(0xffffffffu, mine.x, j + u), take<EXACT>(r[u]));
+                for (int u = 0; u < U; ++u) add(__shfl_sync(0xffffffffu, mine.x, j + u), take<MODE>(r[u]));
                 j += U;
             } else {
                 const T* row = dy + (long long)__shfl_sync(0xffffffffu, mine.y, j) * a.dy_ld;
                 const uint32_t key = __shfl_sync(0xffffffffu, mine.x, j);
-                add(key, gather_block(row, c, a.dim));
+                add(key, MODE == kShift ? gather_block(row, c, a.dim) : load_block<T, MODE>(row, c, a.dim).x);
                 ++j;
             }
         }
@@ -683,17 +713,17 @@ __device__ __forceinline__ void sum_group(const GradArgs& a, const uint2* list, 
     }
 }
 
-template <typename T, bool EXACT>
-__global__ void __launch_bounds__(32 * kSumWarps, EXACT ? 4 : 3) grad_chunks_kernel(GradArgs a) {
+template <typename T, int MODE>
+__global__ void __launch_bounds__(32 * kSumWarps, MODE == kShift ? 3 : 4) grad_chunks_kernel(GradArgs a) {
     __shared__ SumSpace<T, kSumWarps> m;
     mgw_let_next_start();
     if ((int)blockIdx.x < a.zero_blocks) {
-        fill_rows<T, EXACT>(a, blockIdx.x);
+        fill_rows<T, MODE>(a, blockIdx.x);
         return;
     }
     mgw_wait_for_previous();
     const long long task = blockIdx.x - a.zero_blocks, group = task / a.slabs;
-    sum_group<T, EXACT, kSumWarps>(a, a.list, group, (int)(task - group * a.slabs), m);
+    sum_group<T, MODE, kSumWarps>(a, a.list, group, (int)(task - group * a.slabs), m);
 }
 
 // Everything in one launch, for at most 1024 tokens: every slab's block sorts the list for itself and is the only group.
@@ -702,21 +732,21 @@ struct SmallSpace {
     unsigned char rest[];                  // SmallSort, then SumSpace
 };
 
-template <typename T, bool EXACT>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(32 * kSmallWarps) grad_small_kernel(GradArgs a, SortPass p, int passes) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     SmallSpace& m = *reinterpret_cast<SmallSpace*>(dynamic);
     if ((int)blockIdx.x >= a.slabs) {
-        fill_rows<T, EXACT>(a, blockIdx.x - a.slabs);
+        fill_rows<T, MODE>(a, blockIdx.x - a.slabs);
         return;
     }
     if (blockIdx.x > 0) p.status = nullptr;                           // one report is enough
     const uint2* list = sort_in_block(p, passes, m.list, *reinterpret_cast<SmallSort*>(m.rest));
-    sum_group<T, EXACT, kSmallWarps>(a, list, 0, blockIdx.x, *reinterpret_cast<SumSpace<T, kSmallWarps>*>(m.rest));
+    sum_group<T, MODE, kSmallWarps>(a, list, 0, blockIdx.x, *reinterpret_cast<SumSpace<T, kSmallWarps>*>(m.rest));
 }
 
 // Runs that cross borders of groups: the warp of the group in which a run starts adds up its partial sums, for one slab.
-template <typename T, bool EXACT>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a) {
     constexpr int N = per_block<T>(), Q = N / 4, U = 8;               // partial sums in flight, added in their order
     mgw_wait_for_previous();
@@ -761,16 +791,25 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a) {
         acc[4 * q] = x[q].x * a.scale; acc[4 * q + 1] = x[q].y * a.scale;
         acc[4 * q + 2] = x[q].z * a.scale; acc[4 * q + 3] = x[q].w * a.scale;
     }
-    store_blocks<T, EXACT>(static_cast<T*>(a.dw) + (long long)run * a.dim, (slab * 32 + lane) * N, a.dim, mgw_pack<T, N>(acc));
+    store_blocks<T, MODE>(static_cast<T*>(a.dw) + (long long)run * a.dim, column_of<T, MODE>(slab, lane), a.dim, mgw_pack<T, N>(acc));
 }
 
 int element_size(int dtype) { return dtype == MGW_F32 ? 4 : 2; }
 
-// All rows begin on 16-byte boundaries and consist of whole blocks.
-bool whole_blocks(const void* base, long long ld, int dim, int dtype) {
+// How the rows of a matrix can be moved.
+int mode_of(const void* base, long long ld, int dim, int dtype) {
     const int es = element_size(dtype);
-    return (((unsigned long long)(uintptr_t)base | (unsigned long long)(ld * es) | (unsigned long long)((long long)dim * es)) & 15) == 0;
+    const unsigned long long x = (unsigned long long)(uintptr_t)base | (unsigned long long)(ld * es) | (unsigned long long)((long long)dim * es);
+    return (x & 15) == 0 ? kExact : (x & 3) == 0 ? kWords : kShift;
 }
+
+// f<type, mode>(...) for the type and for the mode that suits both matrices
+#define MGW_BY_TYPE(f, mode, ...)                                                                                  \
+    (dtype == MGW_F32   ? ((mode) == kExact ? f<float, kExact>(__VA_ARGS__) : f<float, kWords>(__VA_ARGS__))       \
+     : dtype == MGW_F16 ? ((mode) == kExact   ? f<__half, kExact>(__VA_ARGS__)                                     \
+                           : (mode) == kWords ? f<__half, kWords>(__VA_ARGS__) : f<__half, kShift>(__VA_ARGS__))   \
+                        : ((mode) == kExact   ? f<__nv_bfloat16, kExact>(__VA_ARGS__)                              \
+                           : (mode) == kWords ? f<__nv_bfloat16, kWords>(__VA_ARGS__) : f<__nv_bfloat16, kShift>(__VA_ARGS__)))
 
 // The sort: digits per pass and scratch memory.
 struct SortPlan {
@@ -806,7 +845,8 @@ SumPlan sum_plan(long long n, int dim, int dtype) {
     const int per = 16 / element_size(dtype);
     s.slabs = (dim + 32 * per - 1) / (32 * per);
     // A warp's part of the list: short enough that there are blocks for every SM, long enough that they run as one wave
-    // where that is possible (three or four of them per SM) and that few runs cross its borders.
+    // where that is possible (four of them per SM) and that few runs cross its borders.  16,384 tokens of 10000 x 512: 26 us
+    // as one wave, 30 us as one and three quarters.
     const long long even = (n * s.slabs + kSumWarps * 148 * 4 - 1) / (kSumWarps * 148 * 4);
     s.chunk = (int)(even < 8 ? 8 : even > kMaxChunk ? kMaxChunk : (even + 3) / 4 * 4);
     s.groups = (int)((n + (long long)kSumWarps * s.chunk - 1) / ((long long)kSumWarps * s.chunk));
@@ -826,32 +866,32 @@ int allow_smem(void (*kernel)(P...), size_t bytes, std::atomic<unsigned long lon
     return MGW_OK;
 }
 
-template <typename T, bool EXACT>
+template <typename T, int MODE>
 int launch_small(const GradArgs& a, const SortPass& p, int passes, cudaStream_t stream) {
     static std::atomic<unsigned long long> done{0};
     const size_t rest = sizeof(SmallSort) > sizeof(SumSpace<T, kSmallWarps>) ? sizeof(SmallSort) : sizeof(SumSpace<T, kSmallWarps>);
     const size_t smem = sizeof(SmallSpace) + rest;
-    const int rc = allow_smem(grad_small_kernel<T, EXACT>, smem, done);
+    const int rc = allow_smem(grad_small_kernel<T, MODE>, smem, done);
     if (rc != MGW_OK) return rc;
-    grad_small_kernel<T, EXACT><<<a.slabs + a.zero_blocks, 32 * kSmallWarps, smem, stream>>>(a, p, passes);
+    grad_small_kernel<T, MODE><<<a.slabs + a.zero_blocks, 32 * kSmallWarps, smem, stream>>>(a, p, passes);
     MGW_CUDA_CHECK(cudaGetLastError());
     return MGW_OK;
 }
 
-template <typename T, bool EXACT>
+template <typename T, int MODE>
 int launch_sums(const GradArgs& a, cudaStream_t stream) {
-    const int rc = launch_dependent(grad_chunks_kernel<T, EXACT>, (long long)a.groups * a.slabs + a.zero_blocks, 32 * kSumWarps, 0, stream, a);
+    const int rc = launch_dependent(grad_chunks_kernel<T, MODE>, (long long)a.groups * a.slabs + a.zero_blocks, 32 * kSumWarps, 0, stream, a);
     if (rc != MGW_OK || a.groups == 1) return rc;
-    return launch_dependent(grad_join_kernel<T, EXACT>, ((long long)(a.groups - 1) * a.slabs + 7) / 8, 256, 0, stream, a);
+    return launch_dependent(grad_join_kernel<T, MODE>, ((long long)(a.groups - 1) * a.slabs + 7) / 8, 256, 0, stream, a);
 }
 
-template <typename T, bool EXACT>
+template <typename T, int MODE>
 int launch_fwd(const void* tokens, int wide, long long n, const void* weight, long long ld, long long vocab, int dim, float scale,
                void* out, int* status, cudaStream_t stream) {
-    const int per = 32 * lookup_unroll(EXACT) * per_block<T>(), segments = (dim + (EXACT ? 0 : per_block<T>() - 1) + per - 1) / per;
+    const int per = 32 * lookup_unroll(MODE) * per_block<T>(), segments = (dim + (MODE == kShift ? per_block<T>() - 1 : 0) + per - 1) / per;
     const long long blocks = (n * segments + 7) / 8;
     const unsigned grid = (unsigned)(blocks < 148LL * 64 ? blocks : 148LL * 64);
-    embedding_fwd_kernel<T, EXACT><<<grid, 256, 0, stream>>>(tokens, wide, n, static_cast<const T*>(weight), ld, vocab, dim, scale,
+    embedding_fwd_kernel<T, MODE><<<grid, 256, 0, stream>>>(tokens, wide, n, static_cast<const T*>(weight), ld, vocab, dim, scale,
                                                              static_cast<T*>(out), segments, status);
     MGW_CUDA_CHECK(cudaGetLastError());
     return MGW_OK;
@@ -890,12 +930,8 @@ extern "C" int mgw_embedding_fwd(const void* tokens, int wide, long long n, cons
     if (n == 0) return MGW_OK;
     if (tokens == nullptr || weight == nullptr || out == nullptr || status == nullptr) return MGW_ERR_ARG;
     if (((uintptr_t)weight | (uintptr_t)out) & (element_size(dtype) - 1)) return MGW_ERR_ARG;
-    const bool exact = whole_blocks(weight, ld, dim, dtype) && whole_blocks(out, dim, dim, dtype);
-    cudaStream_t s = (cudaStream_t)stream;
-#define MGW_FWD(T) (exact ? launch_fwd<T, true>(tokens, wide, n, weight, ld, vocab, dim, scale, out, status, s) \
-                          : launch_fwd<T, false>(tokens, wide, n, weight, ld, vocab, dim, scale, out, status, s))
-    return dtype == MGW_F32 ? MGW_FWD(float) : dtype == MGW_F16 ? MGW_FWD(__half) : MGW_FWD(__nv_bfloat16);
-#undef MGW_FWD
+    const int wm = mode_of(weight, ld, dim, dtype), om = mode_of(out, dim, dim, dtype), mode = wm > om ? wm : om;
+    return MGW_BY_TYPE(launch_fwd, mode, tokens, wide, n, weight, ld, vocab, dim, scale, out, status, (cudaStream_t)stream);
 }
 
 extern "C" size_t mgw_embedding_grad_bytes(long long n, long long vocab, int dim, int dtype) {
@@ -922,26 +958,24 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
     a.tokens = tokens; a.wide = wide;
     a.n = n; a.tiles = p.tiles; a.bits = p.bits;
     a.vocab = vocab; a.padding = padding; a.status = status;
-    // Rows without tokens are filled by blocks of the same launch as the sums.  Those of a short list read all tokens and
-    // start while the sort runs; a long list (where every block would read too much) is searched when it is sorted.
+    // Rows without tokens are filled by blocks of the same launch as the sums.  Those of a list of up to 65,536 tokens read
+    // all tokens and start while the sort runs (20,011 tokens of a table of 32,003: 54 us, 63 us when the sorted list is
+    // searched instead); of a longer list every block would read too much.  Four blocks per SM where they read little
+    // (262,144 tokens, searched: 315 us, with one per SM 323), one where each reads a long list.
     GradArgs g = {};
     g.n = n; g.dy = dy; g.dy_ld = dy_ld; g.dw = dw; g.vocab = vocab; g.dim = dim; g.scale = scale;
     g.chunk = q.chunk; g.groups = q.groups; g.slabs = q.slabs;
     g.by_tokens = n <= kClusterList;
     g.tokens = tokens; g.wide = wide; g.padding = padding;
-    const bool exact = whole_blocks(dy, dy_ld, dim, dtype) && whole_blocks(dw, dim, dim, dtype);
+    const int ym = mode_of(dy, dy_ld, dim, dtype), wm = mode_of(dw, dim, dim, dtype), mode = ym > wm ? ym : wm;
     const bool small = n <= kSmallList;
     const int fillers = small ? (q.slabs < 74 ? 148 - q.slabs : 74) : !g.by_tokens || n <= 4096 ? 148 * 4 : 148;
     g.zero_rows = (int)((vocab + fillers - 1) / fillers);
     if (g.zero_rows > kZeroRows) g.zero_rows = kZeroRows;
     g.zero_blocks = (int)((vocab + g.zero_rows - 1) / g.zero_rows);
-#define MGW_BY_TYPE(f, ...)                                                                            \
-    (dtype == MGW_F32   ? (exact ? f<float, true>(__VA_ARGS__) : f<float, false>(__VA_ARGS__))         \
-     : dtype == MGW_F16 ? (exact ? f<__half, true>(__VA_ARGS__) : f<__half, false>(__VA_ARGS__))       \
-                        : (exact ? f<__nv_bfloat16, true>(__VA_ARGS__) : f<__nv_bfloat16, false>(__VA_ARGS__)))
     if (small) {
         g.chunk = (int)((n + kSmallWarps - 1) / kSmallWarps);
-        return MGW_BY_TYPE(launch_small, g, a, p.passes, s);
+        return MGW_BY_TYPE(launch_small, mode, g, a, p.passes, s);
     }
     if (work == nullptr || work_bytes < mgw_embedding_grad_bytes(n, vocab, dim, dtype) || ((uintptr_t)work & 15)) return MGW_ERR_ARG;
     char* at = static_cast<char*>(work);
@@ -974,6 +1008,5 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
     }
     g.list = list[n > kClusterList ? (p.passes - 1) & 1 : 0];
     g.partial = reinterpret_cast<float*>(at);
-    return MGW_BY_TYPE(launch_sums, g, s);
-#undef MGW_BY_TYPE
+    return MGW_BY_TYPE(launch_sums, mode, g, s);
 }

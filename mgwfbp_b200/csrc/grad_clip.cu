@@ -290,7 +290,7 @@ int launch_norm(const Call& c, int norm) {
     return norm == kNorm2 ? launch<CAP, kNorm2>(c) : norm == kNorm1 ? launch<CAP, kNorm1>(c) : launch<CAP, kNormMax>(c);
 }
 
-constexpr int kSmall = 64, kLarge = 1024;                   // kernel arguments of 1.4 KB and 21 KB
+constexpr int kSmall = 64, kLarge = 1024;                   // tensors per launch: kernel arguments of 1.4 KB and 21 KB
 
 int fail(const char* text) {
     mgw_set_last_error(cudaErrorInvalidValue, text, __FILE__, __LINE__);
