@@ -31,7 +31,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxTop = 32;
-constexpr int kThreads = 128;              // 8 blocks per SM; 64 threads: prompts 105 us instead of 99, training 84 instead of 75
+constexpr int kThreads = 128;              // 8 blocks per SM; with 64 threads the first case above takes 105 us, not 99
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;                 // 16-byte vectors of a thread in a batch
 constexpr int kStages = 2;                 // batches of a warp: one in use, one on its way

@@ -44,11 +44,11 @@ def _lib_ready():
 
 class TokenLogProbs(NamedTuple):
     """Per row: log probability of the given token, entropy (natural logarithm), log probabilities and indices of the
-    likeliest tokens (largest first, equal values by the lower index; ``[..., 0]`` when ``top`` is 0)."""
+    likeliest tokens (``[..., top]``, largest first, equal values by the lower index; ``None`` when ``top`` is 0)."""
     logprob: torch.Tensor
     entropy: torch.Tensor
-    top_logprob: torch.Tensor
-    top_tokens: torch.Tensor
+    top_logprob: Optional[torch.Tensor]
+    top_tokens: Optional[torch.Tensor]
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -75,11 +75,12 @@ def _check(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> None:
 
 def _rows(logits: torch.Tensor):
     """The logits as ``[rows, vocabulary]`` with contiguous rows, and the distance between rows."""
-    v = logits.shape[-1]
-    z = logits.reshape(-1, v)
-    if z.stride(1) != 1 and v > 1 or z.shape[0] > 1 and z.stride(0) < v:
-        z = z.contiguous()
-    return z, (z.stride(0) if z.shape[0] > 1 else v)
+    z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    n, v = z.shape
+    ld, step = z.stride()
+    if step != 1 and v > 1 or n > 1 and ld < v:
+        z, ld = z.contiguous(), v
+    return z, (ld if n > 1 else v)
 
 
 def _grad_like(z: torch.Tensor, ld: int) -> torch.Tensor:
@@ -91,32 +92,23 @@ def _grad_like(z: torch.Tensor, ld: int) -> torch.Tensor:
     return torch.empty(n, v, dtype=z.dtype, device=z.device)
 
 
-def _launch_forward(z, ld, tokens, ignore, top, entropy, keep_stats, stream):
-    n, v = z.shape
-    f32 = dict(dtype=torch.float32, device=z.device)
-    logprob = torch.empty(n, **f32)
-    h = torch.empty(n, **f32) if entropy else None
-    stats = torch.empty(n, 2, **f32) if keep_stats else None
-    top_logprob = torch.empty(n, top, **f32) if top else None
-    top_tokens = torch.empty(n, top, dtype=torch.int64, device=z.device) if top else None
-    if n:
-        _lib.check(_lib_ready().mgw_logprob_fwd(z.data_ptr(), ld, n, v, DTYPE_CODES[z.dtype], tokens.data_ptr(),
-                                                tokens.dtype == torch.int64, ignore, logprob.data_ptr(), _ptr(h), _ptr(stats), top,
-                                                _ptr(top_logprob), _ptr(top_tokens), status_words(), stream), 'logprob_fwd')
-        counters.bump('logprob_fwd')
-    return logprob, h, stats, top_logprob, top_tokens
-
-
 def _forward_cuda(logits, tokens, ignore, top, keep_stats):
-    shape = tokens.shape
+    """Log probability, entropy, alternatives, and the rows' statistics for the backward pass."""
+    shape, n, v, device = tokens.shape, tokens.numel(), logits.shape[-1], logits.device
     with device_guard(logits):
         z, ld = _rows(logits)
         tokens = tokens.contiguous()
-        logprob, h, stats, tlp, tt = _launch_forward(z, ld, tokens, ignore, top, True, keep_stats, stream_of(z))
-        if tlp is None:
-            tlp = logprob.new_empty(logprob.shape[0], 0)
-            tt = tlp.to(torch.int64)
-        return logprob.view(shape), h.view(shape), tlp.view(*shape, top), tt.view(*shape, top), stats
+        logprob = torch.empty(shape, dtype=torch.float32, device=device)
+        h = torch.empty(shape, dtype=torch.float32, device=device)
+        stats = torch.empty(n, 2, dtype=torch.float32, device=device) if keep_stats else None
+        tlp = torch.empty(*shape, top, dtype=torch.float32, device=device) if top else None
+        tt = torch.empty(*shape, top, dtype=torch.int64, device=device) if top else None
+        if n:
+            _lib.check(_lib_ready().mgw_logprob_fwd(z.data_ptr(), ld, n, v, DTYPE_CODES[z.dtype], tokens.data_ptr(),
+                                                    tokens.dtype == torch.int64, ignore, logprob.data_ptr(), h.data_ptr(), _ptr(stats),
+                                                    top, _ptr(tlp), _ptr(tt), status_words(), stream_of(z)), 'logprob_fwd')
+            counters.bump('logprob_fwd')
+    return logprob, h, tlp, tt, stats
 
 
 class _TokenLogProbs(torch.autograd.Function):
@@ -125,7 +117,8 @@ class _TokenLogProbs(torch.autograd.Function):
         logprob, h, tlp, tt, stats = _forward_cuda(logits, tokens, ignore, top, True)
         ctx.save_for_backward(logits, tokens, stats, h)
         ctx.ignore = ignore
-        ctx.mark_non_differentiable(tlp, tt)
+        if top:
+            ctx.mark_non_differentiable(tlp, tt)
         ctx.set_materialize_grads(False)
         return logprob, h, tlp, tt
 
@@ -148,7 +141,7 @@ class _TokenLogProbs(torch.autograd.Function):
                                                         _ptr(g2), None, None, 0, 0.0, dz.data_ptr(), dz.stride(0) if n > 1 else v,
                                                         stream_of(z)), 'logprob_bwd')
                 counters.bump('logprob_bwd')
-            return dz.view(logits.shape), None, None, None
+            return dz if logits.dim() == 2 else dz.view(logits.shape), None, None, None
 
 
 def _reference(logits: torch.Tensor, tokens: torch.Tensor, ignore: int, top: int):
@@ -166,10 +159,12 @@ def _reference(logits: torch.Tensor, tokens: torch.Tensor, ignore: int, top: int
     p = logp.exp()
     h = -(p * logp.masked_fill(p == 0, 0.0)).sum(1)
     logprob, h = chosen.masked_fill(pad, 0.0), h.masked_fill(pad, 0.0)
+    s = tokens.shape
+    if not top:
+        return logprob.view(s), h.view(s), None, None
     order = torch.sort(z.detach(), dim=1, descending=True, stable=True).indices[:, :top]
     tlp = logp.detach().gather(1, order).masked_fill(pad.unsqueeze(1), 0.0)
     tt = order.masked_fill(pad.unsqueeze(1), -1)
-    s = tokens.shape
     return logprob.view(s), h.view(s), tlp.view(*s, top), tt.view(*s, top)
 
 
@@ -229,7 +224,7 @@ class _CrossEntropy(torch.autograd.Function):
                                                         g.data_ptr(), work.data_ptr(), written, ctx.expected, dz.data_ptr(),
                                                         dz.stride(0) if n > 1 else v, stream_of(z)), 'cross_entropy_bwd')
                 counters.bump('cross_entropy_bwd')
-            return dz.view(logits.shape), None, None, None, None
+            return dz if logits.dim() == 2 else dz.view(logits.shape), None, None, None, None
 
 
 def cross_entropy(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int = -100, reduction: str = 'mean',

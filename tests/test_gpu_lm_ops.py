@@ -224,6 +224,9 @@ def test_log_probs_and_gradient(rows, vocab, pad, dtype):
         r = token_log_probs(z, t if top % 2 else t.int(), top=top)
         assert_within(r.logprob, *want.logprob(), 'logprob')
         assert_within(r.entropy, *want.entropy(), 'entropy')
+        if top == 0:
+            assert r.top_logprob is None and r.top_tokens is None
+            continue
         v, bound, order = want.top(top)
         assert torch.equal(r.top_tokens, order), top
         assert_within(r.top_logprob, v, bound, 'top')
