@@ -733,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
                 if (part == 0 && warp == 0)
                     for (int k = 1; k < a.splits; ++k) mine = merge_lists(mine, *cluster.map_shared_rank(&block_list[lane], k));
             }
-            if (part == 0 && warp == 0 && lane < a.top) {
+            if (part == 0 && warp == 0 && lane < a.top && mine != 0) {      // key 0 is no entry: never an index
                 const int j = (int)(0xffffffffu - (uint32_t)mine);
                 a.top_tokens[r * a.top + lane] = j;
                 a.top_logprob[r * a.top + lane] = fine ? ln_prob<T>(mgw_to_float(row.z[j]), x.m, log2_s) : mgw_nan();
