@@ -4,11 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
-
-// codes of the C interface
-#define MGW_F32 0
-#define MGW_F16 1
-#define MGW_BF16 2
+#include "lm_api.h"
 
 #ifdef __CUDACC__
 

@@ -8,10 +8,11 @@ loader may build it on demand so that import-time checks still work.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 from typing import Optional
 
-from .build import CHECKED_LIB_PATH, LIB_PATH, build  # noqa: F401  (re-exported)
+from .build import BINDING_PATH, CHECKED_LIB_PATH, LIB_PATH, build  # noqa: F401  (re-exported)
 
 MAX_RANKS = 16
 MAX_CTAS = 296
@@ -82,6 +83,18 @@ def _declare(lib: C.CDLL) -> None:
     lib.mgw_bounds_sgd.argtypes = [C.POINTER(C.c_int)]
     lib.mgw_phase_times.argtypes = [C.POINTER(C.c_ulonglong), C.c_int]
     lib.mgw_s2d_stem_input.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]
+    p, n, i = C.c_void_p, C.c_longlong, C.c_int
+    lib.mgw_token_status.argtypes = [C.POINTER(C.POINTER(C.c_int))]
+    lib.mgw_embedding_fwd.argtypes = [p, i, n, p, n, n, i, i, C.c_float, p, p, p]
+    lib.mgw_embedding_grad_bytes.restype = C.c_size_t
+    lib.mgw_embedding_grad_bytes.argtypes = [n, n, i, i]
+    lib.mgw_embedding_grad.argtypes = [p, n, p, i, n, n, i, i, C.c_float, n, p, p, C.c_size_t, p, p]
+    lib.mgw_logprob_fwd.argtypes = [p, n, n, i, i, p, i, n, p, p, p, i, p, p, p, p]
+    lib.mgw_logprob_bwd.argtypes = [p, n, n, i, i, p, i, n, p, p, p, p, p, p, i, C.c_float, p, n, p]
+    lib.mgw_cross_entropy_fwd.argtypes = [p, n, n, i, i, p, i, n, i, C.c_float, p, p, p, p, n, p, p, p]
+    lib.mgw_grad_clip_bytes.restype = C.c_size_t
+    lib.mgw_grad_clip_bytes.argtypes = [i]
+    lib.mgw_grad_clip.argtypes = [p, p, p, i, i, C.c_double, C.c_double, i, p, C.c_size_t, p, p]
     for name in ('mgw_bn_relu_fwd', 'mgw_bn_relu_bwd', 'mgw_lstm_cell_fwd', 'mgw_lstm_cell_bwd',
                  'mgw_wgrad_gemm', 'mgw_wgrad_gemm_supported', 'mgw_allgather_rows'):
         if hasattr(lib, name):
@@ -111,6 +124,29 @@ def load(allow_build: Optional[bool] = None) -> C.CDLL:
     _declare(lib)
     _lib = lib
     return lib
+
+
+_binding = None
+
+
+def load_binding():
+    """The module of ``csrc/torch_binding.cpp`` with the loaded library's functions bound to it."""
+    global _binding
+    if _binding is None:
+        import torch
+        if not os.path.isfile(BINDING_PATH):
+            raise NativeLibraryError('%s is missing; run `python -m mgwfbp_b200.ops.build`' % BINDING_PATH)
+        spec = importlib.util.spec_from_file_location('_torch_binding', BINDING_PATH)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise NativeLibraryError('could not load %s: %s' % (BINDING_PATH, e)) from e
+        if module.torch_version != torch.__version__:
+            raise NativeLibraryError('%s was built for PyTorch %s, this is %s; run `python -m mgwfbp_b200.ops.build`'
+                                     % (BINDING_PATH, module.torch_version, torch.__version__))
+        _binding = module
+    return _binding
 
 
 def is_checked() -> bool:

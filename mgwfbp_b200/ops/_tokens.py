@@ -1,46 +1,36 @@
 # -*- coding: utf-8 -*-
-"""What the operators on token lists share: type codes, the launch's device and stream, and the status words in which a
-kernel records a token outside the vocabulary."""
+"""What the operators on token lists share: the types, the bound native module, and the status words in which a kernel
+records a token outside the vocabulary."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import torch
 
-from . import _lib
+from . import _lib, counters
 
-DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 _OPS = {1: 'embedding', 2: 'embedding gradient', 3: 'token log probabilities'}
-_same_device = contextlib.nullcontext()
+_FUNCTIONS = ('mgw_last_error', 'mgw_embedding_fwd', 'mgw_embedding_grad_bytes', 'mgw_embedding_grad', 'mgw_logprob_fwd',
+              'mgw_logprob_bwd', 'mgw_cross_entropy_fwd', 'mgw_grad_clip_bytes', 'mgw_grad_clip')
 
 
 class TokenIndexError(IndexError):
     """A kernel met a token outside the vocabulary."""
 
 
-def device_guard(t: torch.Tensor):
-    """Context in which ``t``'s device is the current one (nothing to do when it already is)."""
-    return _same_device if t.get_device() == _current_device() else torch.cuda.device(t.device)
+_native = None
 
 
-def stream_of(t: torch.Tensor) -> int:
-    return _raw_stream(t.get_device())
-
-
-# called with CUDA tensors only, so CUDA is up: no need for the lazy start of torch.cuda.current_device, and the stream's
-# handle alone costs 0.1 us where a Stream object costs 2.2 us
-_current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
-_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def once_differentiable(backward):
-    """As ``torch.autograd.function.once_differentiable``, without its cost where no second derivative can be asked for."""
-    guarded = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
+def native():
+    """The module that allocates, launches and records gradients for CUDA tensors (``csrc/torch_binding.cpp``)."""
+    global _native
+    if _native is None:
+        lib, module = _lib.load(allow_build=False), _lib.load_binding()
+        module.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in _FUNCTIONS}, status_words(), _lib.NativeLibraryError)
+        counters.attach(module.launch_counts)
+        _native = module
+    return _native
 
 
 _words = None
@@ -50,10 +40,8 @@ def status_words() -> int:
     """Address of the process's status words: pinned host memory that every device can write."""
     global _words
     if _words is None:
-        lib = _lib.load(allow_build=False)
         p = C.POINTER(C.c_int)()
-        lib.mgw_token_status.argtypes = [C.POINTER(C.POINTER(C.c_int))]
-        _lib.check(lib.mgw_token_status(C.byref(p)), 'token status')
+        _lib.check(_lib.load(allow_build=False).mgw_token_status(C.byref(p)), 'token status')
         _words = (C.cast(p, C.c_void_p).value, p)
     return _words[0]
 

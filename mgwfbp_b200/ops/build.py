@@ -4,7 +4,8 @@
 ``python -m mgwfbp_b200.ops.build [--verbose] [--force] [--checked]``.  Every ``.cu`` under ``csrc/`` is compiled to
 an object (only when stale) and linked into ``mgwfbp_b200/lib/libmgwfbp_b200.so``.  The CUDA runtime
 is linked statically, so the library only needs the driver at load time and can be loaded in a
-process that also runs PyTorch.
+process that also runs PyTorch.  ``csrc/torch_binding.cpp`` (the autograd nodes and launches of the language-model
+operators) is compiled with the host compiler against the installed PyTorch into ``lib/_torch_binding.so``.
 """
 from __future__ import annotations
 
@@ -13,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from typing import List
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -23,6 +25,9 @@ LIB_PATH = os.path.join(LIB_DIR, 'libmgwfbp_b200.so')
 # the same sources with -DMGW_CHECKED: index checks inside the table-driven kernels (csrc/common.cuh)
 CHECKED_OBJ_DIR = os.path.join(LIB_DIR, 'obj_checked')
 CHECKED_LIB_PATH = os.path.join(LIB_DIR, 'libmgwfbp_b200_checked.so')
+
+BINDING_SRC = os.path.join(SRC_DIR, 'torch_binding.cpp')
+BINDING_PATH = os.path.join(LIB_DIR, '_torch_binding.so')
 
 ARCH_FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a']
 COMMON = ['-O3', '-std=c++17', '-lineinfo', '-Xcompiler', '-fPIC', '--expt-relaxed-constexpr']
@@ -75,6 +80,39 @@ def build(verbose: bool = False, force: bool = False, checked: bool = False) -> 
     return lib_path
 
 
+def build_binding(verbose: bool = False, force: bool = False) -> str:
+    """Compile ``csrc/torch_binding.cpp`` when it, its header or the installed PyTorch has changed."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    stamp = os.path.join(OBJ_DIR, 'torch_binding.version')
+    built_for = ''
+    if os.path.isfile(stamp):
+        with open(stamp) as f:
+            built_for = f.read()
+    if not force and built_for == torch.__version__ and not _stale(BINDING_PATH, [BINDING_SRC, os.path.join(SRC_DIR, 'lm_api.h')]):
+        return BINDING_PATH
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    cuda = os.path.dirname(os.path.dirname(nvcc_path()))
+    system = [os.path.join(root, 'include'), os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
+              sysconfig.get_paths()['include'], os.path.join(cuda, 'include')]
+    cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden',
+           '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch._C._GLIBCXX_USE_CXX11_ABI, '-DTORCH_EXTENSION_NAME=_torch_binding',
+           '-DMGW_TORCH_VERSION="%s"' % torch.__version__, '-I', SRC_DIR]
+    for d in system:
+        cmd += ['-isystem', d]
+    cmd += [BINDING_SRC, '-L' + os.path.join(root, 'lib'), '-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch_python', '-o', BINDING_PATH]
+    if verbose:
+        print(' '.join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+    if res.returncode != 0:
+        raise RuntimeError('%s failed on %s' % (cmd[0], BINDING_SRC))
+    with open(stamp, 'w') as f:
+        f.write(torch.__version__)
+    return BINDING_PATH
+
+
 if __name__ == '__main__':
     ap = argparse.ArgumentParser()
     ap.add_argument('--verbose', action='store_true')
@@ -82,3 +120,4 @@ if __name__ == '__main__':
     ap.add_argument('--checked', action='store_true', help='build libmgwfbp_b200_checked.so (kernels verify their indices)')
     a = ap.parse_args()
     print(build(a.verbose, a.force, a.checked))
+    print(build_binding(a.verbose, a.force))

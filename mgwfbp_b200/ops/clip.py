@@ -10,30 +10,14 @@ not part of the fused momentum-SGD update (``ops.sgd``).  On CPU tensors the sam
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
-from array import array
-from typing import Iterable, List, Union
+from typing import Iterable, List, Optional, Union
 
 import torch
 
-from . import _lib, counters
-from ._tokens import DTYPE_CODES, device_guard, stream_of
+from ._tokens import DTYPES, native
 
 _NORMS = {2.0: 0, 1.0: 1, math.inf: 2}
-_ready = None
-
-
-def _lib_ready():
-    global _ready
-    if _ready is None:
-        lib = _lib.load(allow_build=False)
-        lib.mgw_grad_clip_bytes.restype = C.c_size_t
-        lib.mgw_grad_clip_bytes.argtypes = [C.c_int]
-        lib.mgw_grad_clip.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_double, C.c_double, C.c_int, C.c_void_p,
-                                      C.c_size_t, C.c_void_p, C.c_void_p]
-        _ready = lib
-    return _ready
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -50,8 +34,7 @@ def _dense(t: torch.Tensor) -> bool:
 
 def supported(grads: List[torch.Tensor]) -> bool:
     """Whether :func:`clip_grad_norm_` runs the kernels on these gradients."""
-    return bool(grads) and all(g.is_cuda and g.layout == torch.strided and g.dtype in DTYPE_CODES and g.device == grads[0].device
-                               and _dense(g) for g in grads)
+    return bool(grads) and grads[0].is_cuda and native().clip_supported(grads)
 
 
 def _norm_code(norm_type: float) -> int:
@@ -68,46 +51,18 @@ def _check(grads: List[torch.Tensor]) -> None:
             raise TypeError('gradients must be dense floating-point tensors, got %s %s' % (g.dtype, g.layout))
         if g.device != first:
             raise ValueError('gradients are on %s and %s: clip the gradients of one device' % (first, g.device))
-        if g.is_cuda and g.dtype not in DTYPE_CODES:
+        if g.is_cuda and g.dtype not in DTYPES:
             raise TypeError('gradients must be float32, float16 or bfloat16, got %s' % g.dtype)
         if not _dense(g):
             raise ValueError('a gradient of shape %s has strides %s: its elements do not fill one stretch of memory'
                              % (tuple(g.shape), g.stride()))
 
 
-_tensor = torch.Tensor
-
-
-def _codes(grads: List[torch.Tensor]):
-    """Type codes of the gradients when all of them are contiguous, on one GPU and of a type the kernels know, else None.
-    (Models have hundreds of gradients: five C calls for each, no Python frame.)"""
-    try:
-        codes = bytes([DTYPE_CODES[g.dtype] for g in grads])
-        if grads[0].is_cuda and len(set(map(_tensor.get_device, grads))) == 1 and all(map(_tensor.is_contiguous, grads)):
-            return codes
-    except (KeyError, RuntimeError):                      # another type; sparse
-        pass
-    return None
-
-
-def _launch(grads: List[torch.Tensor], codes: bytes, code: int, scale: float, max_norm: float, clip: bool) -> torch.Tensor:
-    lib, n, first = _lib_ready(), len(grads), grads[0]
-    ptrs, numels = array('Q', map(_tensor.data_ptr, grads)), array('q', map(_tensor.numel, grads))
-    with device_guard(first):
-        out = torch.empty((), dtype=torch.float32, device=first.device)
-        need = lib.mgw_grad_clip_bytes(n)
-        work = torch.empty(need, dtype=torch.uint8, device=first.device)
-        rc = lib.mgw_grad_clip(ptrs.buffer_info()[0], numels.buffer_info()[0], codes, n, code, scale, max_norm, clip, work.data_ptr(), need,
-                               out.data_ptr(), stream_of(first))
-        if rc == 2:
-            raise ValueError('grad_clip: %s' % lib.mgw_last_error().decode(errors='replace'))
-        _lib.check(rc, 'grad_clip')
-        if clip:
-            for g in [g for g in grads if g.requires_grad]:        # part of a graph (create_graph): it has changed in place
-                torch.autograd.graph.increment_version(g)
-        counters.bump('grad_norm', (n + 1023) // 1024)
-        counters.bump('grad_scale' if clip else 'grad_norm_finish', (n + 1023) // 1024 if clip else 1)
-    return out
+def _kernels(tensors: List[torch.Tensor], parameters: bool, code: int, scale: float, max_norm: float, clip: bool) -> Optional[torch.Tensor]:
+    """Norm (and scaling) by the kernels of ``tensors`` or of their gradients; ``None`` where those are not for them."""
+    if not any(t.is_cuda for t in tensors):
+        return None
+    return native().clip_grads(tensors, parameters, code, scale, max_norm, clip)
 
 
 def _reference_norm(grads: List[torch.Tensor], norm_type: float, scale: float) -> torch.Tensor:
@@ -130,13 +85,11 @@ def grad_norm(grads: Iterable[torch.Tensor], norm_type: float = 2.0, grad_scale:
     code, scale, grads = _norm_code(norm_type), _check_scale(grad_scale), list(grads)
     if not grads:
         return torch.zeros(())
-    codes = _codes(grads)
-    if codes is None:
+    norm = _kernels(grads, False, code, scale, 0.0, False)
+    if norm is None:
         _check(grads)
-        if not grads[0].is_cuda:
-            return _reference_norm(grads, float(norm_type), scale).float()
-        codes = bytes(DTYPE_CODES[g.dtype] for g in grads)
-    return _launch(grads, codes, code, scale, 0.0, False)
+        norm = _reference_norm(grads, float(norm_type), scale).float()
+    return norm
 
 
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -150,22 +103,18 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     code, scale, max_norm = _norm_code(norm_type), _check_scale(grad_scale), float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError('max_norm must not be negative, got %r' % (max_norm,))
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    if error_if_nonfinite:
+        norm = grad_norm([p.grad for p in parameters if p.grad is not None], norm_type, scale)
+        if not math.isfinite(float(norm)):
+            raise RuntimeError('The total norm of order %s for the gradients is non-finite, so they cannot be clipped' % (norm_type,))
+    norm = _kernels(parameters, True, code, scale, max_norm, True)
+    if norm is not None:
+        return norm
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.zeros(())
-    codes = _codes(grads)
-    if codes is None:
-        _check(grads)
-        if grads[0].is_cuda:
-            codes = bytes(DTYPE_CODES[g.dtype] for g in grads)
-    if error_if_nonfinite:
-        norm = grad_norm(grads, norm_type, scale)
-        if not math.isfinite(float(norm)):
-            raise RuntimeError('The total norm of order %s for the gradients is non-finite, so they cannot be clipped' % (norm_type,))
-    if codes is not None:
-        return _launch(grads, codes, code, scale, max_norm, True)
+    _check(grads)
     norm = _reference_norm(grads, float(norm_type), scale)
     factor = float(scale * torch.clamp(max_norm / (norm + 1e-6), max=1.0))
     for g in {(g.data_ptr(), g.numel()): g for g in grads}.values():

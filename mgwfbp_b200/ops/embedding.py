@@ -12,33 +12,14 @@ functions run plain PyTorch operations.
 """
 from __future__ import annotations
 
-import ctypes as C
-import functools
 from typing import Optional
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
-from . import _lib, counters
-from ._tokens import (DTYPE_CODES, TokenIndexError, check_status, check_status_nosync, check_tokens, device_guard,  # noqa: F401
-                      once_differentiable, status_words, stream_of)
-
-_ready = None
-
-
-def _lib_ready():
-    global _ready
-    if _ready is None:
-        lib = _lib.load(allow_build=False)
-        lib.mgw_embedding_fwd.argtypes = [C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong, C.c_longlong, C.c_int, C.c_int,
-                                          C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]
-        lib.mgw_embedding_grad_bytes.restype = C.c_size_t
-        lib.mgw_embedding_grad_bytes.argtypes = [C.c_longlong, C.c_longlong, C.c_int, C.c_int]
-        lib.mgw_embedding_grad.argtypes = [C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_longlong, C.c_longlong, C.c_int, C.c_int,
-                                           C.c_float, C.c_longlong, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]
-        _ready = lib
-    return _ready
+from ._tokens import DTYPES, TokenIndexError, check_status, check_status_nosync, check_tokens, native  # noqa: F401
 
 
 def _check(tokens: torch.Tensor, weight: torch.Tensor) -> None:
@@ -48,7 +29,7 @@ def _check(tokens: torch.Tensor, weight: torch.Tensor) -> None:
     if tokens.device != weight.device:
         raise ValueError('tokens are on %s, weight is on %s' % (tokens.device, weight.device))
     if weight.is_cuda:
-        if weight.dtype not in DTYPE_CODES:
+        if weight.dtype not in DTYPES:
             raise TypeError('weight must be float32, float16 or bfloat16, got %s' % weight.dtype)
         _check_sizes(tokens.numel(), *weight.shape)
 
@@ -64,25 +45,6 @@ def _padding(padding_idx: Optional[int], vocab: int) -> int:
     if not -vocab <= padding_idx < vocab:
         raise ValueError('padding_idx %d is outside a vocabulary of %d' % (padding_idx, vocab))
     return padding_idx % vocab
-
-
-def _forward(tokens: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
-    vocab, dim = weight.shape
-    if not weight.is_cuda:
-        out = F.embedding(tokens, weight)
-        return out if scale == 1.0 else (out.double() * scale).to(out.dtype)
-    if weight.stride(1) != 1 or weight.stride(0) < dim:
-        weight = weight.contiguous()
-    tokens = tokens.contiguous()
-    with device_guard(weight):
-        out = torch.empty(*tokens.shape, dim, dtype=weight.dtype, device=weight.device)
-        n = tokens.numel()
-        if n:
-            _lib.check(_lib_ready().mgw_embedding_fwd(tokens.data_ptr(), tokens.dtype == torch.int64, n, weight.data_ptr(),
-                                                      weight.stride(0), vocab, dim, DTYPE_CODES[weight.dtype], scale, out.data_ptr(),
-                                                      status_words(), stream_of(weight)), 'embedding_fwd')
-            counters.bump('embedding_fwd')
-    return out
 
 
 def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, num_embeddings: int, scale: float = 1.0,
@@ -104,50 +66,20 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, num_embeddings: int
         keep = ids != padding
         dw.index_add_(0, ids[keep], rows[keep].double())
         return (dw * scale).to(grad.dtype)
-    if grad.dtype not in DTYPE_CODES:
+    if grad.dtype not in DTYPES:
         raise TypeError('grad must be float32, float16 or bfloat16, got %s' % grad.dtype)
     _check_sizes(n, num_embeddings, dim)
-    return _grad_cuda(grad, tokens, num_embeddings, scale, padding)
+    return native().embedding_grad(grad, tokens, num_embeddings, scale, padding)
 
 
-@functools.lru_cache(maxsize=256)
-def _work_bytes(n: int, vocab: int, dim: int, code: int) -> int:
-    return _lib_ready().mgw_embedding_grad_bytes(n, vocab, dim, code)
-
-
-def _grad_cuda(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: float, padding: int) -> torch.Tensor:
-    n, dim = tokens.numel(), grad.shape[-1]
-    rows = grad.reshape(n, dim)
-    if n and (rows.stride(1) != 1 or (n > 1 and rows.stride(0) < dim)):
-        rows = rows.contiguous()
-    tokens = tokens.contiguous()
-    code = DTYPE_CODES[grad.dtype]
-    with device_guard(grad):
-        dw = torch.empty(vocab, dim, dtype=grad.dtype, device=grad.device)
-        need = _work_bytes(n, vocab, dim, code)
-        work = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
-        _lib.check(_lib_ready().mgw_embedding_grad(rows.data_ptr(), rows.stride(0) if n > 1 else dim, tokens.data_ptr(),
-                                                   tokens.dtype == torch.int64, n, vocab, dim, code, scale, padding, dw.data_ptr(),
-                                                   None if work is None else work.data_ptr(), need, status_words(), stream_of(grad)), 'embedding_grad')
-        counters.bump('embedding_grad')
-    return dw
-
-
-class _Embedding(torch.autograd.Function):
+class _EmbeddingCPU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding):
         ctx.save_for_backward(tokens)
-        ctx.scale, ctx.padding, ctx.vocab, ctx.dtype = scale, padding, weight.shape[0], weight.dtype
-        return _forward(tokens, weight, scale)
+        ctx.scale, ctx.padding, ctx.vocab = scale, padding, weight.shape[0]
+        out = F.embedding(tokens, weight)
+        return out if scale == 1.0 else (out.double() * scale).to(out.dtype)
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        (tokens,) = ctx.saved_tensors
-        return None, _grad_cuda(dy, tokens, ctx.vocab, ctx.scale, ctx.padding), None, None
-
-
-class _EmbeddingCPU(_Embedding):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
@@ -161,9 +93,9 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     lie further apart than their width.  ``padding_idx`` only matters to the gradient: that row gets none."""
     _check(tokens, weight)
     padding, scale = _padding(padding_idx, weight.shape[0]), float(scale)
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return (_Embedding if weight.is_cuda else _EmbeddingCPU).apply(tokens, weight, scale, padding)
-    return _forward(tokens, weight, scale)
+    if weight.is_cuda:
+        return native().embedding(tokens, weight, scale, padding)
+    return _EmbeddingCPU.apply(tokens, weight, scale, padding)
 
 
 class FusedEmbedding(nn.Embedding):
@@ -179,7 +111,7 @@ class FusedEmbedding(nn.Embedding):
         self.scale = float(scale)
 
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
-        if self.weight.is_cuda and self.weight.dtype not in DTYPE_CODES:
+        if self.weight.is_cuda and self.weight.dtype not in DTYPES:
             return super().forward(tokens) * self.scale
         return embedding(tokens, self.weight, self.scale, self.padding_idx)
 

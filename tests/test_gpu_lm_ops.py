@@ -73,8 +73,9 @@ def test_embedding_every_width_and_alignment(dtype):
 
 def test_embedding_gradient_writes_nothing_else():
     """The rows behind and before the result stay as they were."""
-    from mgwfbp_b200.ops import embedding as emb
-    lib = emb._lib_ready()
+    from mgwfbp_b200.ops import _lib
+    from mgwfbp_b200.ops._tokens import status_words
+    lib = _lib.load(allow_build=False)
     for n in (6, 3000, 70000):
         for dim, shift in ((37, 3), (64, 0)):
             t = torch.randint(0, 50, (n,), device='cuda')
@@ -84,7 +85,7 @@ def test_embedding_gradient_writes_nothing_else():
             need = lib.mgw_embedding_grad_bytes(n, 50, dim, 0)
             work = torch.empty(need, dtype=torch.uint8, device='cuda')
             assert lib.mgw_embedding_grad(dy.data_ptr(), dim, t.data_ptr(), 1, n, 50, dim, 0, 1.0, -1, dw.data_ptr(),
-                                          work.data_ptr() if need else None, need, emb.status_words(),
+                                          work.data_ptr() if need else None, need, status_words(),
                                           torch.cuda.current_stream().cuda_stream) == 0
             want, bound = oracle_grad(dy, t, 50, 1.0)
             assert_within(dw.view(50, dim), want, bound, 'dw')
@@ -680,3 +681,86 @@ def test_refusals_on_the_gpu():
         x = w.float().requires_grad_()
         (g,) = torch.autograd.grad(token_log_probs(x[:1], t).logprob.sum(), x, create_graph=True)
         torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.parametrize('kind', ['embedding', 'log_probs', 'cross_entropy'])
+def test_gradients_are_differentiable_once(kind):
+    """A second derivative raises an error, also where the incoming gradient has no graph of its own."""
+    from mgwfbp_b200.ops.embedding import embedding
+    from mgwfbp_b200.ops.logprob import cross_entropy, token_log_probs
+    t = torch.tensor([1, 3, 3], device='cuda')
+    w = torch.randn(5, 4, device='cuda', requires_grad=True)
+    z = torch.randn(3, 7, device='cuda', requires_grad=True)
+    if kind == 'embedding':
+        up = torch.randn(3, 4, device='cuda', requires_grad=True)
+        leaf, out = w, (embedding(t, w) * up).sum()
+    else:
+        leaf, out = z, token_log_probs(z, t).logprob.sum() if kind == 'log_probs' else cross_entropy(z, t)
+    (plain,) = torch.autograd.grad(out, leaf, retain_graph=True)
+    assert not plain.requires_grad
+    (g,) = torch.autograd.grad(out, leaf, create_graph=True)
+    assert torch.equal(g, plain) and g.requires_grad
+    with pytest.raises(RuntimeError, match='differentiate twice'):
+        (g.square().sum() + out).backward()
+
+
+def test_graph_is_released_and_guards_its_inputs():
+    """Nothing outlives the graph, a released graph is refused, and so are inputs that changed since."""
+    import gc
+    from mgwfbp_b200.ops.embedding import embedding
+    from mgwfbp_b200.ops.logprob import cross_entropy, token_log_probs
+    t = torch.randint(0, 1000, (512,), device='cuda')
+    w = torch.randn(1000, 256, device='cuda', requires_grad=True)
+    z = torch.randn(512, 1000, device='cuda', requires_grad=True)
+
+    def forward():
+        return [embedding(t, w), token_log_probs(z, t, top=3).logprob, token_log_probs(z, t).entropy, cross_entropy(z, t)]
+    for out in forward():                                      # the first calls' own memory
+        out.sum().backward()
+    w.grad = z.grad = out = None
+    gc.collect()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for turn in range(2):
+        for out in forward():
+            if turn:
+                total = out.sum()
+                total.backward()
+                with pytest.raises(RuntimeError, match='second time'):
+                    total.backward()
+                total = None
+        w.grad = z.grad = out = None                           # (with turn 0: graphs that never ran backward)
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() == before
+    for k in (1, 2, 3):
+        out = forward()[k]
+        with torch.no_grad():
+            z.mul_(1.0)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            out.sum().backward()
+    out = forward()[0]
+    t.add_(0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        out.sum().backward()
+
+
+def test_clip_marks_gradients_as_changed():
+    from mgwfbp_b200.ops.clip import clip_grad_norm_
+    p = torch.nn.Parameter(torch.zeros(8, device='cuda'))
+    p.grad = torch.ones(8, device='cuda')
+    x = torch.ones(8, device='cuda', requires_grad=True)
+    y = (x * p.grad).sum()                                     # saves the gradient
+    clip_grad_norm_([p], 0.5)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward()
+
+
+def test_clip_with_parameters_on_the_host_that_have_no_gradient():
+    from mgwfbp_b200.ops.clip import clip_grad_norm_
+    from mgwfbp_b200.ops import counters
+    ps = [torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3, device='cuda'))]
+    ps[1].grad = torch.full((3,), 2.0, device='cuda')
+    before = counters.snapshot()
+    clip_grad_norm_(iter(ps), 1.0)
+    assert counters.diff(before) == {'grad_norm': 1, 'grad_scale': 1}
+    assert abs(ps[1].grad.norm().item() - 1.0) < 1e-5          # max_norm / (norm + 1e-6): 3e-7 below 1

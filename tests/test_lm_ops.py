@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from lm_oracle import Rows, assert_within, embedding_grad as oracle_grad, half_step, tiny
-from mgwfbp_b200.ops import clip, embedding as emb, logprob as lp
+from mgwfbp_b200.ops import _lib, clip, embedding as emb, logprob as lp
 
 
 # ---------------------------------------------------------------------------------------------------------- embedding
@@ -205,7 +205,7 @@ def test_clip_refusals():
 # ------------------------------------------------------------------------------------------- the native entry points
 # Every call below is refused by the host code before anything is launched.
 def test_native_embedding_refuses_bad_arguments():
-    lib = emb._lib_ready()
+    lib = _lib.load(allow_build=False)
     buf = (C.c_int * 64)()
     p = C.addressof(buf)
     ok = dict(tokens=p, wide=0, n=4, weight=p, ld=4, vocab=8, dim=4, dtype=0, scale=1.0, out=p, status=p, stream=None)
@@ -222,7 +222,7 @@ def test_native_embedding_refuses_bad_arguments():
 
 
 def test_native_logprob_refuses_bad_arguments():
-    lib = lp._lib_ready()
+    lib = _lib.load(allow_build=False)
     buf = (C.c_int * 64)()
     p = C.addressof(buf)
     ok = dict(z=p, ld=8, rows=2, vocab=8, dtype=0, tokens=p, wide=0, ignore=-100, logprob=p, entropy=p, stats=p, top=2, tlp=p, tt=p,
@@ -242,7 +242,7 @@ def test_native_logprob_refuses_bad_arguments():
 
 
 def test_native_clip_refuses_bad_arguments():
-    lib = clip._lib_ready()
+    lib = _lib.load(allow_build=False)
     buf = (C.c_double * 4096)()
     work, need = C.addressof(buf), lib.mgw_grad_clip_bytes(2)
     assert need <= C.sizeof(buf)
