@@ -13,15 +13,16 @@
 // shared memory.  What bounds it is the number of instructions per logit, so the inner loop works on pairs: maxima and
 // the lower limit on packed bf16 or fp16, multiply-adds and sums on packed fp32.
 //
-// Measured (device time): 4099 rows of 50,261 bf16 logits with 20 alternatives 94 us (413 MB; 67 us without the
-// alternatives, 63 us is the floor), 700 x 10,000 fp32 with 5 of them 10.5 us (7.3 without), 2048 x 32,000 bf16 26 us and its
+// Measured (device time): 4099 rows of 50,261 bf16 logits with 20 alternatives 89 us (413 MB; 67 us without the
+// alternatives, 63 us is the floor), 700 x 10,000 fp32 with 5 of them 9.6 us (7.3 without), 2048 x 32,000 bf16 26 us and its
 // gradient 49 us (5.3 TB/s).  Mean loss with gradient of 8192 x 131,072 bf16 780 us (4.3 GB, 5.5 TB/s: logits once from
 // memory, once from L2, gradient once to memory), 700 x 10,000 fp32 21 us.  Before the pairs, with 256 threads per block
 // and plain loads, these were 184, 15, 38 + 61 and 1017 us.
 //
 // The likeliest tokens come out of the same pass.  Every thread knows the largest of its logits, so a value that K
-// threads reach is a lower bound for the K-th largest; every warp keeps the maximum of each 128 vectors that it read,
-// and only those that reach the bound are looked at again (from L2).  What reaches the bound is sorted, 32 keys to a warp.
+// threads reach is a lower bound for the K-th largest; it also keeps the maximum of every four vectors that it read, and
+// only those that reach the bound are looked at again (from L2).  What reaches the bound is sorted, 32 keys to a warp.  With
+// maxima of the warps' 128 vectors in their place two fifths of a row were read again: 94 us in the first case.
 #include <cooperative_groups.h>
 #include "api.h"
 #include "dtypes.cuh"
@@ -36,7 +37,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;                 // 16-byte vectors of a thread in a batch
 constexpr int kStages = 2;                 // batches of a warp: one in use, one on its way
 constexpr int kBatch = 32 * kUnroll;       // vectors that a warp reads at a time
-constexpr int kMaxima = 128;               // maxima that a warp keeps; neighbouring batches share one beyond that
+constexpr int kCellBytes = 8192;           // maxima of the threads' batches; neighbouring batches share one beyond that
 constexpr int kCandidates = 512;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -355,33 +356,34 @@ struct Row {
 
 constexpr size_t kRingBytes = (size_t)kWarps * kStages * kBatch * 16;
 
-struct TopSpace {
-    float maxima[kWarps][kMaxima];         // of the batches of a warp
+// Maxima of a thread's batches: 32 of them for 16-bit types, 16 for fp32.
+template <typename T> constexpr int kCells = kCellBytes / (kThreads * (int)sizeof(T));
+
+struct TopSpace {                          // in the memory of the ring, which the scan no longer needs
     uint32_t most[kThreads];               // order of the threads' maxima, 0: the thread has no vector
     uint32_t floor;                        // a lower bound of the order of the K-th largest value
     unsigned long long list[kWarps][32];
     unsigned long long candidate[kCandidates];
     int n_candidates;
 };
+static_assert(sizeof(TopSpace) <= kRingBytes, "it takes the ring's place");
 
-// Sums of this block's part of the row; with TOP also the batches' maxima and the thread's own (most: minus infinity
-// where it has no vector).
+// Sums of this block's part of the row; with TOP also the maxima of the thread's batches and of all its vectors (most: minus
+// infinity where it has none).
 template <typename T, bool ENT, bool TOP>
-__device__ __forceinline__ Sums scan_row(const Row<T>& row, uint4* ring, int shift, TopSpace* top, float& most) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ Sums scan_row(const Row<T>& row, uint4* ring, int shift, T* cells, float& most) {
+    const int lane = threadIdx.x & 31;
     Sums a;
     a.m = Fast<T>::start;
     a.M = __fmul_rn(a.m, kLog2e);
     a.s = a.u = pair(0.f, 0.f);
     most = -INFINITY;
     int batch = 0;
-    auto note = [&](float m) {                                       // the batch's maximum
+    float in_cell = -INFINITY;
+    auto note = [&](float m) {
         most = max_nan(most, m);
-        const float w = warp_max_nan(m);
-        if (lane == 0) {
-            float* to = &top->maxima[warp][batch >> shift];
-            *to = (batch & ((1 << shift) - 1)) == 0 ? w : max_nan(*to, w);
-        }
+        in_cell = (batch & ((1 << shift) - 1)) == 0 ? m : max_nan(in_cell, m);
+        cells[(batch >> shift) * kThreads + threadIdx.x] = mgw_from_float<T>(in_cell);
         ++batch;
     };
     row.for_batches(ring, [&](int, const uint4 (&r)[kUnroll]) {
@@ -526,10 +528,22 @@ __device__ __noinline__ Key top_by_lists(const Row<T>& row, float floor, TopSpac
     return join_lists(mine, t);
 }
 
+// Element q of the values in r, by selection: an indexed array would live in memory.
+template <typename T>
+__device__ __forceinline__ T element(const uint4 (&r)[kUnroll], int q) {
+    static_assert(kUnroll == 4, "sixteen words");
+    const int w = q * (int)sizeof(T) >> 2;
+    const uint4 a = w & 4 ? r[1] : r[0], b = w & 4 ? r[3] : r[2], c = w & 8 ? b : a;
+    const uint32_t lo = w & 1 ? c.y : c.x, hi = w & 1 ? c.w : c.z;
+    uint32_t word = w & 2 ? hi : lo;
+    if (sizeof(T) == 2 && (q & 1)) word >>= 16;
+    return *reinterpret_cast<const T*>(&word);
+}
+
 // The 32 largest keys of this block's part of the row (at least the `top` largest are right), in the lanes of the first
 // warp, the largest first.
 template <typename T>
-__device__ __forceinline__ Key find_top(const Row<T>& row, int top, int shift, float most, TopSpace* t) {
+__device__ __forceinline__ Key find_top(const Row<T>& row, int top, int shift, float most, const T* cells, TopSpace* t) {
     constexpr int N = Vec<T>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // the bound: a value that `top` of the threads' maxima reach, the upper 16 bits of its order found by one warp, two at a
@@ -560,31 +574,27 @@ __device__ __forceinline__ Key find_top(const Row<T>& row, int top, int shift, f
     __syncthreads();
     const uint32_t low = t->floor;
     const float floor = value_of_key(low);
-    int batch = 0;
-    for (int i0 = row.v0 + warp * kBatch; i0 < row.v1; i0 += kWarps * kBatch, ++batch) {
-        if (t->maxima[warp][batch >> shift] < floor) continue;
-        uint32_t hits = 0;                                           // which of the lane's kUnroll * N values reach the bound
+    if (!(most < floor)) {                                           // not many more than `top` threads
+        int batch = 0;
+        for (int i0 = row.v0 + warp * kBatch + lane; i0 < row.v1; i0 += kWarps * kBatch, ++batch) {
+            if (mgw_to_float(cells[(batch >> shift) * kThreads + threadIdx.x]) < floor) continue;
+            uint4 r[kUnroll];
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            const int i = i0 + k * 32 + lane;
-            if (i >= row.v1) continue;
-            float f[N];
-            mgw_unpack<T, N>(row.vec(i), f);
+            for (int k = 0; k < kUnroll; ++k)
+                if (i0 + k * 32 < row.v1) r[k] = row.vec(i0 + k * 32);
+            uint32_t hits = 0;                                       // which of the kUnroll * N values reach the bound
 #pragma unroll
-            for (int e = 0; e < N; ++e) hits |= f[e] < floor ? 0u : 1u << (k * N + e);
-        }
-        int before = __popc(hits);
+            for (int k = 0; k < kUnroll; ++k) {
+                float f[N];
+                mgw_unpack<T, N>(r[k], f);
+                if (i0 + k * 32 >= row.v1) continue;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before += v;
-        }
-        int at = 0;
-        if (lane == 31) at = atomicAdd(&t->n_candidates, before);    // the order does not matter: keys are sorted
-        at = __shfl_sync(0xffffffffu, at, 31) + before - __popc(hits);
-        for (; hits != 0; hits &= hits - 1, ++at) {
-            const int q = __ffs(hits) - 1, j = row.head + (i0 + q / N * 32 + lane) * N + q % N;
-            if (at < kCandidates) t->candidate[at] = key_of(mgw_to_float(row.z[j]), j);
+                for (int e = 0; e < N; ++e) hits |= f[e] < floor ? 0u : 1u << (k * N + e);
+            }
+            for (; hits != 0; hits &= hits - 1) {
+                const int q = __ffs(hits) - 1, at = atomicAdd(&t->n_candidates, 1);      // the order does not matter: keys are sorted
+                if (at < kCandidates) t->candidate[at] = key_of(mgw_to_float(element<T>(r, q)), row.head + (i0 + q / N * 32) * N + q % N);
+            }
         }
     }
     const int j = row.edge(threadIdx.x);
@@ -678,7 +688,7 @@ template <typename T, bool ENT, bool TOP, bool LOSS>
 __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     uint4* ring = reinterpret_cast<uint4*>(dynamic);
-    TopSpace* top = reinterpret_cast<TopSpace*>(dynamic + kRingBytes);       // only with TOP
+    T* cells = reinterpret_cast<T*>(dynamic + kRingBytes);           // only with TOP
     __shared__ Stats parts[kWarps];
     __shared__ Stats of_block;
     __shared__ Key block_list[kMaxTop];
@@ -703,9 +713,9 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
     } else {
         int shift = 0;
         if (TOP)
-            while (((row.v1 - row.v0) / (kWarps * kBatch) >> shift) >= kMaxima) ++shift;
+            while (((row.v1 - row.v0) / (kWarps * kBatch) >> shift) >= kCells<T>) ++shift;
         float most;
-        Stats x = block_join<ENT>(scan_row<T, ENT, TOP>(row, ring, shift, top, most), parts);
+        Stats x = block_join<ENT>(scan_row<T, ENT, TOP>(row, ring, shift, cells, most), parts);
         if (a.splits > 1) {
             cg::cluster_group cluster = cg::this_cluster();
             if (threadIdx.x == 0) of_block = x;
@@ -725,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
         }
         if (TOP) {
             const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-            Key mine = find_top(row, a.top, shift, most, top);
+            Key mine = find_top(row, a.top, shift, most, cells, reinterpret_cast<TopSpace*>(ring));
             if (a.splits > 1) {
                 cg::cluster_group cluster = cg::this_cluster();
                 if (warp == 0) block_list[lane] = mine;
@@ -868,7 +878,7 @@ bool bad_rows(const void* z, long long ld, long long rows, int vocab, int dtype,
 
 template <typename T, bool ENT, bool TOP, bool LOSS>
 int launch_fwd(const RowArgs& a, cudaStream_t stream) {
-    const size_t smem = kRingBytes + (TOP ? sizeof(TopSpace) : 0);
+    const size_t smem = kRingBytes + (TOP ? kCellBytes : 0);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * a.splits));
     cfg.blockDim = dim3(kThreads);
