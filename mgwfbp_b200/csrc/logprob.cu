@@ -13,16 +13,18 @@
 // shared memory.  What bounds it is the number of instructions per logit, so the inner loop works on pairs: maxima and
 // the lower limit on packed bf16 or fp16, multiply-adds and sums on packed fp32.
 //
-// Measured (device time): 4099 rows of 50,261 bf16 logits with 20 alternatives 89 us (413 MB; 67 us without the
+// Measured (device time): 4099 rows of 50,261 bf16 logits with 20 alternatives 84 us (413 MB; 67 us without the
 // alternatives, 63 us is the floor), 700 x 10,000 fp32 with 5 of them 9.6 us (7.3 without), 2048 x 32,000 bf16 26 us and its
 // gradient 49 us (5.3 TB/s).  Mean loss with gradient of 8192 x 131,072 bf16 780 us (4.3 GB, 5.5 TB/s: logits once from
 // memory, once from L2, gradient once to memory), 700 x 10,000 fp32 21 us.  Before the pairs, with 256 threads per block
 // and plain loads, these were 184, 15, 38 + 61 and 1017 us.
 //
-// The likeliest tokens come out of the same pass.  Every thread knows the largest of its logits, so a value that K
-// threads reach is a lower bound for the K-th largest; it also keeps the maximum of every four vectors that it read, and
-// only those that reach the bound are looked at again (from L2).  What reaches the bound is sorted, 32 keys to a warp.  With
-// maxima of the warps' 128 vectors in their place two fifths of a row were read again: 94 us in the first case.
+// The likeliest tokens come out of the same pass.  Every thread knows the largest of its logits, so the K-th largest of the
+// maxima of 64 pairs of threads, found by sorting them in one warp, is a lower bound for the K-th largest logit.  Every thread
+// also keeps the maximum of each four vectors that it read, and only those that reach the bound are looked at again (from
+// L2).  What reaches the bound is sorted, 32 keys to a warp.  In the first case: with maxima of the warps' 128 vectors two
+// fifths of a row were read again, 94 us; with the bound searched bit by bit, and with the logits of the chosen and of the
+// likeliest tokens read at the end, 88 us.
 #include <cooperative_groups.h>
 #include "api.h"
 #include "dtypes.cuh"
@@ -467,26 +469,28 @@ typedef unsigned long long Key;
 
 __device__ __forceinline__ Key key_of(float v, int index) { return ((Key)order_key(v) << 32) | (0xffffffffu - (uint32_t)index); }
 
-__device__ __forceinline__ Key sort_lanes(Key x) {                   // bitonic, descending
+template <typename K>
+__device__ __forceinline__ K sort_lanes(K x) {                       // bitonic, descending
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
         for (int o = size >> 1; o > 0; o >>= 1) {
-            const Key y = __shfl_xor_sync(0xffffffffu, x, o);
+            const K y = __shfl_xor_sync(0xffffffffu, x, o);
             const bool larger = ((lane & o) == 0) == ((lane & size) == 0);
             x = larger == (y > x) ? y : x;
         }
     return x;
 }
 
-__device__ __forceinline__ Key merge_lists(Key a, Key b) {           // both descending: the 32 largest of the 64
+template <typename K>
+__device__ __forceinline__ K merge_lists(K a, K b) {                 // both descending: the 32 largest of the 64
     const int lane = threadIdx.x & 31;
-    const Key y = __shfl_sync(0xffffffffu, b, 31 - lane);
-    Key x = a > y ? a : y;
+    const K y = __shfl_sync(0xffffffffu, b, 31 - lane);
+    K x = a > y ? a : y;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const Key z = __shfl_xor_sync(0xffffffffu, x, o);
+        const K z = __shfl_xor_sync(0xffffffffu, x, o);
         x = ((lane & o) == 0) == (z > x) ? z : x;
     }
     return x;
@@ -546,29 +550,14 @@ template <typename T>
 __device__ __forceinline__ Key find_top(const Row<T>& row, int top, int shift, float most, const T* cells, TopSpace* t) {
     constexpr int N = Vec<T>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // the bound: a value that `top` of the threads' maxima reach, the upper 16 bits of its order found by one warp, two at a
-    // time (three counts of at most 128 fit into one sum)
+    // the bound: the value that `top` of 64 pairs of threads reach, by sorting the pairs' maxima
     t->most[threadIdx.x] = row.v0 + warp * kBatch + lane < row.v1 ? order_key(most) : 0u;
     if (threadIdx.x == 0) t->n_candidates = 0;
     __syncthreads();
     if (warp == 0) {
-        static_assert(kThreads < 256, "a count has 8 bits");
-        uint32_t key[kWarps], bound = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) key[w] = t->most[w * 32 + lane];
-#pragma unroll
-        for (int bit = 30; bit >= 16; bit -= 2) {
-            uint32_t n = 0;
-#pragma unroll
-            for (int q = 1; q <= 3; ++q)
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) n += key[w] >= (bound | (uint32_t)q << bit) ? 1u << (8 * (q - 1)) : 0u;
-            n = __reduce_add_sync(0xffffffffu, n);
-            if ((int)(n & 0xff) >= top) {                            // fewer reach the larger ones
-                const uint32_t q = (int)(n >> 16 & 0xff) >= top ? 3u : (int)(n >> 8 & 0xff) >= top ? 2u : 1u;
-                bound |= q << bit;
-            }
-        }
+        static_assert(kWarps == 4 && kMaxTop == 32, "two sorted lists of 32 become one");
+        const uint32_t a = sort_lanes(max(t->most[lane], t->most[64 + lane])), b = sort_lanes(max(t->most[32 + lane], t->most[96 + lane]));
+        const uint32_t bound = __shfl_sync(0xffffffffu, merge_lists(a, b), top - 1);
         if (lane == 0) t->floor = bound;
     }
     __syncthreads();
@@ -696,6 +685,9 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
     const long long r = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
     const long long t = mgw_token(a.tokens, a.wide, r);
     const Row<T> row(static_cast<const T*>(a.z) + r * a.ld, a.vocab, part, a.splits);
+    const bool valid = t >= 0 && t < a.vocab;
+    T chosen = mgw_from_float<T>(0.f);                               // read now, so that nothing waits for it at the end
+    if (part == 0 && threadIdx.x == 0 && valid && t != a.ignore) chosen = row.z[t];
     if (t == a.ignore) {                                             // all blocks of the cluster leave
         if (part == 0) {
             if (threadIdx.x == 0) {
@@ -726,10 +718,9 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
         if (careful<T>(x.m)) x = careful_row(row.z, a.vocab, parts);
         const bool fine = fabsf(x.m) < INFINITY;
         const float log2_s = log2f(x.s);
-        const bool valid = t >= 0 && t < a.vocab;
         if (part == 0 && threadIdx.x == 0) {
             if (!valid) mgw_report_token(a.status, MGW_OP_LOGPROB, r, t);
-            a.logprob[r] = valid && fine ? ln_prob<T>(mgw_to_float(row.z[t]), x.m, log2_s) : mgw_nan();
+            a.logprob[r] = valid && fine ? ln_prob<T>(mgw_to_float(chosen), x.m, log2_s) : mgw_nan();
             if (ENT && a.entropy) a.entropy[r] = fine ? kLn2 * (log2_s - x.u / x.s) : mgw_nan();
             if (a.stats) a.stats[r] = make_float2(fine ? x.m : mgw_nan(), log2_s);
         }
@@ -746,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
             if (part == 0 && warp == 0 && lane < a.top && mine != 0) {      // key 0 is no entry: never an index
                 const int j = (int)(0xffffffffu - (uint32_t)mine);
                 a.top_tokens[r * a.top + lane] = j;
-                a.top_logprob[r * a.top + lane] = fine ? ln_prob<T>(mgw_to_float(row.z[j]), x.m, log2_s) : mgw_nan();
+                a.top_logprob[r * a.top + lane] = fine ? ln_prob<T>(value_of_key((uint32_t)(mine >> 32)), x.m, log2_s) : mgw_nan();
             }
         }
         if (LOSS) mgw_wait_for_previous();                               // the count of rows
