@@ -7,7 +7,8 @@
 // however often a single word occurs -- and a warp adds up the rows of one chunk for 512 bytes of columns.  A run of equal
 // tokens inside a chunk is stored at once.  A run that crosses the borders of chunks is put together in the order of the
 // chunks, in shared memory within a block and through fp32 partial sums and a second launch between blocks.  Rows that no
-// token names are filled with zeros by other blocks of the same launch, beside the sort where they can.
+// token names are filled with zeros by other blocks of the same launch, beside the sort where they can; or the
+// sort runs beside a long lookup, whose launch then leaves the sorted list for the gradient.
 //
 // Everything here is bound by memory once the lists are long: 262,144 rows of 2048 bf16 values of a table of 131,072 take
 // 221 us to look up (1.3 GB, 6.0 TB/s) and 305 us to add up (1.6 GB, 5.3 TB/s; of it 40 us are the sort, which has nothing
@@ -192,7 +193,7 @@ constexpr int lookup_unroll(int mode) { return mode == kShift ? 5 : 4; }
 template <typename T, int MODE>
 __global__ void __launch_bounds__(256, 3)
 embedding_fwd_kernel(const void* __restrict__ tokens, int wide, long long n, const T* __restrict__ weight, long long ld,
-                     long long vocab, int dim, float scale, T* __restrict__ out, int segments, int* status) {
+                     long long vocab, int dim, float scale, T* __restrict__ out, int segments, int beside_sort, int* status) {
     constexpr int N = per_block<T>(), U = lookup_unroll(MODE);
     const int lane = threadIdx.x & 31;
     const long long warps = (long long)gridDim.x * (blockDim.x >> 5);
@@ -231,6 +232,8 @@ embedding_fwd_kernel(const void* __restrict__ tokens, int wide, long long n, con
                 if (c + 32 * N * k < dim) put(gather_block(src, c + 32 * N * k, dim), c + 32 * N * k);
         }
     }
+    // the sort was launched first and may still run: what follows this launch in the stream follows the sort too
+    if (beside_sort && blockIdx.x == gridDim.x - 1) mgw_wait_for_previous();
 }
 
 // -------------------------------------------------------------------------------------------------------------- sort
@@ -247,14 +250,14 @@ struct SortPass {
     long long n;
     int tiles, shift, bits;
     long long vocab, padding;
-    int* status;
+    int* status;               // may be null: nothing is reported
 };
 
 __device__ __forceinline__ uint2 sort_entry(const SortPass& p, long long i, bool report) {
     if (p.in != nullptr) return p.in[i];
     const long long t = mgw_token(p.tokens, p.wide, i);
     if (t < 0 || t >= p.vocab) {
-        if (report) mgw_report_token(p.status, MGW_OP_EMBEDDING_GRAD, i, t);
+        if (report && p.status != nullptr) mgw_report_token(p.status, MGW_OP_EMBEDDING_GRAD, i, t);
         return make_uint2((uint32_t)p.vocab, (uint32_t)i);
     }
     return make_uint2(t == p.padding ? (uint32_t)p.vocab : (uint32_t)t, (uint32_t)i);
@@ -879,26 +882,53 @@ int launch_small(const GradArgs& a, const SortPass& p, int passes, cudaStream_t 
 }
 
 template <typename T, int MODE>
-int launch_sums(const GradArgs& a, cudaStream_t stream) {
-    const int rc = launch_dependent(grad_chunks_kernel<T, MODE>, (long long)a.groups * a.slabs + a.zero_blocks, 32 * kSumWarps, 0, stream, a);
-    if (rc != MGW_OK || a.groups == 1) return rc;
+int launch_sums(const GradArgs& a, bool behind_sort, cudaStream_t stream) {
+    const long long grid = (long long)a.groups * a.slabs + a.zero_blocks;
+    if (behind_sort) {
+        const int rc = launch_dependent(grad_chunks_kernel<T, MODE>, grid, 32 * kSumWarps, 0, stream, a);
+        if (rc != MGW_OK) return rc;
+    } else {                                                         // some other kernel is before it: start when that is done
+        grad_chunks_kernel<T, MODE><<<(unsigned)grid, 32 * kSumWarps, 0, stream>>>(a);
+        MGW_CUDA_CHECK(cudaGetLastError());
+    }
+    if (a.groups == 1) return MGW_OK;
     return launch_dependent(grad_join_kernel<T, MODE>, ((long long)(a.groups - 1) * a.slabs + 7) / 8, 256, 0, stream, a);
 }
 
 template <typename T, int MODE>
 int launch_fwd(const void* tokens, int wide, long long n, const void* weight, long long ld, long long vocab, int dim, float scale,
-               void* out, int* status, cudaStream_t stream) {
+               void* out, bool beside_sort, int* status, cudaStream_t stream) {
     const int per = 32 * lookup_unroll(MODE) * per_block<T>(), segments = (dim + (MODE == kShift ? per_block<T>() - 1 : 0) + per - 1) / per;
     const long long blocks = (n * segments + 7) / 8;
     const unsigned grid = (unsigned)(blocks < 148LL * 64 ? blocks : 148LL * 64);
+    if (beside_sort)
+        return launch_dependent(embedding_fwd_kernel<T, MODE>, grid, 256, 0, stream, tokens, wide, n, static_cast<const T*>(weight), ld, vocab,
+                                dim, scale, static_cast<T*>(out), segments, 1, status);
     embedding_fwd_kernel<T, MODE><<<grid, 256, 0, stream>>>(tokens, wide, n, static_cast<const T*>(weight), ld, vocab, dim, scale,
-                                                             static_cast<T*>(out), segments, status);
+                                                             static_cast<T*>(out), segments, 0, status);
     MGW_CUDA_CHECK(cudaGetLastError());
     return MGW_OK;
 }
 
 bool bad_sizes(long long n, long long vocab, int dim, int dtype) {
     return n < 0 || n > 0x7fffffffLL || vocab < 1 || vocab > 0x7ffffffeLL || dim < 1 || dim > (1 << 30) || dtype < MGW_F32 || dtype > MGW_BF16;
+}
+
+int launch_cluster_sort(const SortPass& a, int passes, cudaStream_t stream) {
+    static std::atomic<unsigned long long> done{0};
+    const int rc = allow_smem(sort_cluster_kernel, sizeof(ClusterSmem), done);
+    if (rc != MGW_OK) return rc;
+    sort_cluster_kernel<<<kCluster, kClusterThreads, sizeof(ClusterSmem), stream>>>(a, passes);
+    MGW_CUDA_CHECK(cudaGetLastError());
+    return MGW_OK;
+}
+
+SortPass sort_of(const void* tokens, int wide, long long n, long long vocab, long long padding, const SortPlan& p, int* status) {
+    SortPass a = {};
+    a.tokens = tokens; a.wide = wide;
+    a.n = n; a.tiles = p.tiles; a.bits = p.bits;
+    a.vocab = vocab; a.padding = padding; a.status = status;
+    return a;
 }
 
 }  // namespace
@@ -924,14 +954,36 @@ extern "C" int mgw_token_status(int** out) {
     return MGW_OK;
 }
 
+// The sort of a list that one cluster takes needs 8 SMs and 10 to 30 us, mostly waiting.  Beside a lookup that is as long it
+// costs nothing; otherwise the zeros of the gradient are a better thing to do meanwhile.  Lookup and gradient, with the sort
+// beside the lookup and beside the zeros: 20,011 x 1023 fp16 of 32,003 60 and 69 us, 65,536 x 2048 bf16 of 32,000 137 and 155,
+// 16,384 x 512 fp32 of 10,000 32 and 37; but 4096 x 768 bf16 of 50,000 31 and 25, 1500 x 1500 fp32 of 10,000 27 and 23 (sort
+// 10 us, lookup 3 us).  Lists of up to 1024 are sorted where they are added up, those above 65,536 by six launches there.
+constexpr long long kLongLookup = 32LL << 20;                          // bytes that the lookup writes
+
+extern "C" size_t mgw_embedding_order_bytes(long long n, long long vocab, int dim, int dtype) {
+    if (bad_sizes(n, vocab, dim, dtype) || n <= kSmallList || n > kClusterList || n * dim * element_size(dtype) < kLongLookup) return 0;
+    return sort_plan(n, vocab).list_bytes;
+}
+
 extern "C" int mgw_embedding_fwd(const void* tokens, int wide, long long n, const void* weight, long long ld, long long vocab,
-                                 int dim, int dtype, float scale, void* out, int* status, void* stream) {
+                                 int dim, int dtype, float scale, void* out, void* order, long long padding, int* status,
+                                 void* stream) {
     if (bad_sizes(n, vocab, dim, dtype) || ld < dim) return MGW_ERR_ARG;
     if (n == 0) return MGW_OK;
     if (tokens == nullptr || weight == nullptr || out == nullptr || status == nullptr) return MGW_ERR_ARG;
     if (((uintptr_t)weight | (uintptr_t)out) & (element_size(dtype) - 1)) return MGW_ERR_ARG;
     const int wm = mode_of(weight, ld, dim, dtype), om = mode_of(out, dim, dim, dtype), mode = wm > om ? wm : om;
-    return MGW_BY_TYPE(launch_fwd, mode, tokens, wide, n, weight, ld, vocab, dim, scale, out, status, (cudaStream_t)stream);
+    if (order != nullptr) {
+        if (mgw_embedding_order_bytes(n, vocab, dim, dtype) == 0 || ((uintptr_t)order & 15)) return MGW_ERR_ARG;
+        const SortPlan p = sort_plan(n, vocab);
+        SortPass a = sort_of(tokens, wide, n, vocab, padding, p, nullptr);              // the lookup reports
+        a.out = static_cast<uint2*>(order);
+        const int rc = launch_cluster_sort(a, p.passes, (cudaStream_t)stream);
+        if (rc != MGW_OK) return rc;
+    }
+    return MGW_BY_TYPE(launch_fwd, mode, tokens, wide, n, weight, ld, vocab, dim, scale, out, order != nullptr, status,
+                       (cudaStream_t)stream);
 }
 
 extern "C" size_t mgw_embedding_grad_bytes(long long n, long long vocab, int dim, int dtype) {
@@ -942,8 +994,8 @@ extern "C" size_t mgw_embedding_grad_bytes(long long n, long long vocab, int dim
 }
 
 extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* tokens, int wide, long long n, long long vocab, int dim,
-                                  int dtype, float scale, long long padding, void* dw, void* work, size_t work_bytes, int* status,
-                                  void* stream) {
+                                  int dtype, float scale, long long padding, const void* order, void* dw, void* work, size_t work_bytes,
+                                  int* status, void* stream) {
     if (bad_sizes(n, vocab, dim, dtype) || dw == nullptr) return MGW_ERR_ARG;
     cudaStream_t s = (cudaStream_t)stream;
     if (n == 0) {
@@ -954,22 +1006,21 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
     if (((uintptr_t)dy | (uintptr_t)dw) & (element_size(dtype) - 1)) return MGW_ERR_ARG;
     const SortPlan p = sort_plan(n, vocab);
     const SumPlan q = sum_plan(n, dim, dtype);
-    SortPass a = {};
-    a.tokens = tokens; a.wide = wide;
-    a.n = n; a.tiles = p.tiles; a.bits = p.bits;
-    a.vocab = vocab; a.padding = padding; a.status = status;
+    SortPass a = sort_of(tokens, wide, n, vocab, padding, p, status);
+    if (order != nullptr && (mgw_embedding_order_bytes(n, vocab, dim, dtype) == 0 || ((uintptr_t)order & 15))) return MGW_ERR_ARG;
     // Rows without tokens are filled by blocks of the same launch as the sums.  Those of a list of up to 65,536 tokens read
     // all tokens and start while the sort runs (20,011 tokens of a table of 32,003: 54 us, 63 us when the sorted list is
     // searched instead); of a longer list every block would read too much.  Four blocks per SM where they read little
-    // (262,144 tokens, searched: 315 us, with one per SM 323), one where each reads a long list.
+    // (262,144 tokens, searched: 315 us, with one per SM 323), one where each reads a long list, two where the list is sorted
+    // already (32,768 x 1024 bf16 of 131,072: 92 us, 101 with one, 90 with four; 20,011 x 1023 fp16 of 32,003: 60, 60, 64).
     GradArgs g = {};
     g.n = n; g.dy = dy; g.dy_ld = dy_ld; g.dw = dw; g.vocab = vocab; g.dim = dim; g.scale = scale;
     g.chunk = q.chunk; g.groups = q.groups; g.slabs = q.slabs;
-    g.by_tokens = n <= kClusterList;
+    g.by_tokens = n <= kClusterList && order == nullptr;
     g.tokens = tokens; g.wide = wide; g.padding = padding;
     const int ym = mode_of(dy, dy_ld, dim, dtype), wm = mode_of(dw, dim, dim, dtype), mode = ym > wm ? ym : wm;
     const bool small = n <= kSmallList;
-    const int fillers = small ? (q.slabs < 74 ? 148 - q.slabs : 74) : !g.by_tokens || n <= 4096 ? 148 * 4 : 148;
+    const int fillers = small ? (q.slabs < 74 ? 148 - q.slabs : 74) : order != nullptr ? 148 * 2 : !g.by_tokens || n <= 4096 ? 148 * 4 : 148;
     g.zero_rows = (int)((vocab + fillers - 1) / fillers);
     if (g.zero_rows > kZeroRows) g.zero_rows = kZeroRows;
     g.zero_blocks = (int)((vocab + g.zero_rows - 1) / g.zero_rows);
@@ -987,12 +1038,10 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
     a.out = list[0];
     a.counts = reinterpret_cast<uint32_t*>(at); at += p.counts_bytes;
     a.totals = reinterpret_cast<uint32_t*>(at); at += p.totals_bytes;
-    if (n <= kClusterList) {
-        static std::atomic<unsigned long long> done{0};
-        const int rc = allow_smem(sort_cluster_kernel, sizeof(ClusterSmem), done);
+    if (order != nullptr) {                                          // mgw_embedding_fwd has sorted the tokens
+    } else if (n <= kClusterList) {
+        const int rc = launch_cluster_sort(a, p.passes, s);
         if (rc != MGW_OK) return rc;
-        sort_cluster_kernel<<<kCluster, kClusterThreads, sizeof(ClusterSmem), s>>>(a, p.passes);
-        MGW_CUDA_CHECK(cudaGetLastError());
     } else {
         const int bins = 1 << p.bits;
         const size_t hist_smem = (size_t)bins * 4, scatter_smem = (size_t)bins * 4 + (size_t)bins * 2 * (kSortThreads / 32);
@@ -1006,7 +1055,7 @@ extern "C" int mgw_embedding_grad(const void* dy, long long dy_ld, const void* t
             if (rc != MGW_OK) return rc;
         }
     }
-    g.list = list[n > kClusterList ? (p.passes - 1) & 1 : 0];
+    g.list = order != nullptr ? static_cast<const uint2*>(order) : list[n > kClusterList ? (p.passes - 1) & 1 : 0];
     g.partial = reinterpret_cast<float*>(at);
-    return MGW_BY_TYPE(launch_sums, mode, g, s);
+    return MGW_BY_TYPE(launch_sums, mode, g, order == nullptr, s);
 }

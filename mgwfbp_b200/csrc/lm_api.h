@@ -13,12 +13,16 @@ extern "C" {
 // dtype: MGW_F32 / MGW_F16 / MGW_BF16; tokens: int32 (wide = 0) or int64 (wide = 1).  A token outside
 // [0, vocab) is recorded in `status` (mgw_token_status) and gives a row of NaN, or no contribution to the gradient.
 int mgw_token_status(int** words_out);                               // 8 pinned words, one block per process
+// order: null, or memory of mgw_embedding_order_bytes() (0: not for these sizes) in which the tokens are left sorted for the
+// gradient, without the token `padding`.
+size_t mgw_embedding_order_bytes(long long n, long long vocab, int dim, int dtype);
 int mgw_embedding_fwd(const void* tokens, int wide, long long n, const void* weight, long long ld, long long vocab, int dim, int dtype,
-                      float scale, void* out, int* status, void* stream);
+                      float scale, void* out, void* order, long long padding, int* status, void* stream);
 size_t mgw_embedding_grad_bytes(long long n, long long vocab, int dim, int dtype);      // scratch memory of the call below
-// dw [vocab, dim] is written whole; rows of the token `padding` (-1: none) stay zero.
+// dw [vocab, dim] is written whole; rows of the token `padding` (-1: none) stay zero.  order: null, or what the lookup left.
 int mgw_embedding_grad(const void* dy, long long dy_ld, const void* tokens, int wide, long long n, long long vocab, int dim, int dtype,
-                       float scale, long long padding, void* dw, void* work, size_t work_bytes, int* status, void* stream);
+                       float scale, long long padding, const void* order, void* dw, void* work, size_t work_bytes, int* status,
+                       void* stream);
 
 // ---- log probabilities, entropy, likeliest tokens, cross entropy (logprob.cu) -------------------------
 // stats: [rows][2] largest logit m and log2 of the sum of exp(z - m), for the backward pass (may be null).

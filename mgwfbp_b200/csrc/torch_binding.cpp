@@ -37,6 +37,7 @@ using torch::autograd::variable_list;
 
 struct Library {
     const char* (*last_error)(void) = nullptr;
+    decltype(&mgw_embedding_order_bytes) embedding_order_bytes = nullptr;
     decltype(&mgw_embedding_fwd) embedding_fwd = nullptr;
     decltype(&mgw_embedding_grad_bytes) embedding_grad_bytes = nullptr;
     decltype(&mgw_embedding_grad) embedding_grad = nullptr;
@@ -131,7 +132,8 @@ Tensor once_differentiable(Tensor g, bool wanted) {
 }
 
 // ------------------------------------------------------------------------------------------------------- embedding
-Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, double scale) {
+// order: where it is given and the sizes are such, it becomes the sorted list for the gradient.
+Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding, Tensor* order) {
     need(weight, tokens);
     at::NoGradGuard no_grad;
     Place on(weight);
@@ -139,14 +141,18 @@ Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, double scal
     const Tensor ids = tokens.contiguous();
     Tensor out = at::empty(with_last(tokens.sizes(), w.width), w.t.options());
     if (ids.numel() == 0) return out;
+    if (order != nullptr)
+        if (const size_t bytes = lib.embedding_order_bytes(ids.numel(), w.n, (int)w.width, type_code(w.t)))
+            *order = at::empty({(int64_t)bytes}, w.t.options().dtype(at::kByte));
     check(lib.embedding_fwd(ids.const_data_ptr(), wide(ids), ids.numel(), w.t.const_data_ptr(), w.ld, w.n, (int)w.width, type_code(w.t),
-                            (float)scale, out.mutable_data_ptr(), lib.status, on.stream),
+                            (float)scale, out.mutable_data_ptr(), order != nullptr && order->defined() ? order->mutable_data_ptr() : nullptr,
+                            padding, lib.status, on.stream),
           "embedding_fwd");
     count(kEmbeddingFwd);
     return out;
 }
 
-Tensor embedding_grad(const Tensor& dy, const Tensor& tokens, int64_t vocab, double scale, int64_t padding) {
+Tensor embedding_gradient(const Tensor& dy, const Tensor& tokens, int64_t vocab, double scale, int64_t padding, const Tensor& order) {
     need(dy, tokens);
     at::NoGradGuard no_grad;
     Place on(dy);
@@ -157,14 +163,19 @@ Tensor embedding_grad(const Tensor& dy, const Tensor& tokens, int64_t vocab, dou
     const size_t bytes = lib.embedding_grad_bytes(g.n, vocab, (int)g.width, code);
     if (bytes) work = at::empty({(int64_t)bytes}, dy.options().dtype(at::kByte));
     check(lib.embedding_grad(g.t.const_data_ptr(), g.ld, ids.const_data_ptr(), wide(ids), g.n, vocab, (int)g.width, code, (float)scale,
-                             padding, dw.mutable_data_ptr(), bytes ? work.mutable_data_ptr() : nullptr, bytes, lib.status, on.stream),
+                             padding, order.defined() ? order.const_data_ptr() : nullptr, dw.mutable_data_ptr(), bytes ? work.mutable_data_ptr() : nullptr, bytes, lib.status, on.stream),
           "embedding_grad");
     count(kEmbeddingGrad);
     return dw;
 }
 
+Tensor embedding_grad(const Tensor& dy, const Tensor& tokens, int64_t vocab, double scale, int64_t padding) {
+    return embedding_gradient(dy, tokens, vocab, scale, padding, Tensor());
+}
+
 struct EmbeddingBackward : Node {
     SavedVariable tokens;
+    Tensor order;
     int64_t vocab = 0, padding = -1;
     double scale = 1.0;
 
@@ -172,20 +183,23 @@ struct EmbeddingBackward : Node {
         std::lock_guard<std::mutex> lock(mutex_);
         const Tensor& dy = grads[0];
         if (!dy.defined()) return {Tensor()};
-        return {once_differentiable(embedding_grad(dy, tokens.unpack(), vocab, scale, padding), differentiable(dy))};
+        return {once_differentiable(embedding_gradient(dy, tokens.unpack(), vocab, scale, padding, order), differentiable(dy))};
     }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
         tokens.reset_data();
+        order.reset();
     }
     std::string name() const override { return "EmbeddingBackward"; }
 };
 
 Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
-    Tensor out = embedding_forward(tokens, weight, scale);
-    if (differentiable(weight)) {
+    const bool train = differentiable(weight);
+    Tensor order, out = embedding_forward(tokens, weight, scale, padding, train ? &order : nullptr);
+    if (train) {
         auto node = node_for<EmbeddingBackward>(weight);
         node->tokens = SavedVariable(tokens, false);
+        node->order = order;
         node->vocab = weight.size(0);
         node->padding = padding;
         node->scale = scale;
@@ -418,6 +432,7 @@ PyObject* error_class = PyExc_RuntimeError;                     // kept for the 
 
 void bind(const py::dict& addresses, uintptr_t status, const py::object& error) {
     take(lib.last_error, addresses, "mgw_last_error");
+    take(lib.embedding_order_bytes, addresses, "mgw_embedding_order_bytes");
     take(lib.embedding_fwd, addresses, "mgw_embedding_fwd");
     take(lib.embedding_grad_bytes, addresses, "mgw_embedding_grad_bytes");
     take(lib.embedding_grad, addresses, "mgw_embedding_grad");

@@ -85,10 +85,12 @@ def _declare(lib: C.CDLL) -> None:
     lib.mgw_s2d_stem_input.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]
     p, n, i = C.c_void_p, C.c_longlong, C.c_int
     lib.mgw_token_status.argtypes = [C.POINTER(C.POINTER(C.c_int))]
-    lib.mgw_embedding_fwd.argtypes = [p, i, n, p, n, n, i, i, C.c_float, p, p, p]
+    lib.mgw_embedding_order_bytes.restype = C.c_size_t
+    lib.mgw_embedding_order_bytes.argtypes = [n, n, i, i]
+    lib.mgw_embedding_fwd.argtypes = [p, i, n, p, n, n, i, i, C.c_float, p, p, n, p, p]
     lib.mgw_embedding_grad_bytes.restype = C.c_size_t
     lib.mgw_embedding_grad_bytes.argtypes = [n, n, i, i]
-    lib.mgw_embedding_grad.argtypes = [p, n, p, i, n, n, i, i, C.c_float, n, p, p, C.c_size_t, p, p]
+    lib.mgw_embedding_grad.argtypes = [p, n, p, i, n, n, i, i, C.c_float, n, p, p, p, C.c_size_t, p, p]
     lib.mgw_logprob_fwd.argtypes = [p, n, n, i, i, p, i, n, p, p, p, i, p, p, p, p]
     lib.mgw_logprob_bwd.argtypes = [p, n, n, i, i, p, i, n, p, p, p, p, p, p, i, C.c_float, p, n, p]
     lib.mgw_cross_entropy_fwd.argtypes = [p, n, n, i, i, p, i, n, i, C.c_float, p, p, p, p, n, p, p, p]

@@ -11,7 +11,7 @@ from . import _lib, counters
 
 DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 _OPS = {1: 'embedding', 2: 'embedding gradient', 3: 'token log probabilities'}
-_FUNCTIONS = ('mgw_last_error', 'mgw_embedding_fwd', 'mgw_embedding_grad_bytes', 'mgw_embedding_grad', 'mgw_logprob_fwd',
+_FUNCTIONS = ('mgw_last_error', 'mgw_embedding_order_bytes', 'mgw_embedding_fwd', 'mgw_embedding_grad_bytes', 'mgw_embedding_grad', 'mgw_logprob_fwd',
               'mgw_logprob_bwd', 'mgw_cross_entropy_fwd', 'mgw_grad_clip_bytes', 'mgw_grad_clip')
 
 

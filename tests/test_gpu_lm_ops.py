@@ -84,7 +84,7 @@ def test_embedding_gradient_writes_nothing_else():
             dw = store[5 * dim + shift:55 * dim + shift]
             need = lib.mgw_embedding_grad_bytes(n, 50, dim, 0)
             work = torch.empty(need, dtype=torch.uint8, device='cuda')
-            assert lib.mgw_embedding_grad(dy.data_ptr(), dim, t.data_ptr(), 1, n, 50, dim, 0, 1.0, -1, dw.data_ptr(),
+            assert lib.mgw_embedding_grad(dy.data_ptr(), dim, t.data_ptr(), 1, n, 50, dim, 0, 1.0, -1, None, dw.data_ptr(),
                                           work.data_ptr() if need else None, need, status_words(),
                                           torch.cuda.current_stream().cuda_stream) == 0
             want, bound = oracle_grad(dy, t, 50, 1.0)
@@ -764,3 +764,57 @@ def test_clip_with_parameters_on_the_host_that_have_no_gradient():
     clip_grad_norm_(iter(ps), 1.0)
     assert counters.diff(before) == {'grad_norm': 1, 'grad_scale': 1}
     assert abs(ps[1].grad.norm().item() - 1.0) < 1e-5          # max_norm / (norm + 1e-6): 3e-7 below 1
+
+
+@pytest.mark.parametrize('n,dim', [(5000, 131), (1024, 16500), (1025, 16500), (40000, 451), (65536, 260), (65537, 260)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_embedding_sorted_beside_the_lookup(n, dim, dtype):
+    """The gradient through the graph, whose tokens the lookup's launch has sorted, is the gradient of the plain call bit for bit,
+    whatever runs before and behind it in the stream, also twice and with padding and tokens outside."""
+    from mgwfbp_b200.ops.embedding import check_status, embedding, embedding_grad
+    from mgwfbp_b200.ops._tokens import TokenIndexError
+    gen = torch.Generator(device='cuda').manual_seed(n)
+    vocab = 777
+    w = torch.randn(vocab, dim, device='cuda', generator=gen).to(dtype).requires_grad_()
+    dy = torch.randn(n, dim, device='cuda', generator=gen).to(dtype)
+    for turn in range(4):
+        t = torch.randint(0, vocab, (n,), device='cuda', generator=gen)
+        out = embedding(t, w, 0.5, 3)
+        assert torch.equal(out, (w.detach()[t].float() * 0.5).to(dtype))
+        order_of_release = [torch.full((n,), 9, dtype=torch.int64, device='cuda') for _ in range(3)]     # memory moves on
+        (dw,) = torch.autograd.grad(out, w, dy, retain_graph=True)
+        (again,) = torch.autograd.grad(out, w, dy)
+        want = embedding_grad(dy, t, vocab, 0.5, 3)
+        assert torch.equal(dw, want) and torch.equal(again, want)
+        del order_of_release
+    t[n // 2] = vocab
+    (dw,) = torch.autograd.grad(embedding(t, w, 0.5, 3), w, dy)
+    with pytest.raises(TokenIndexError, match='embedding: token 777 at position %d' % (n // 2)):
+        check_status()
+    want = embedding_grad(dy, t, vocab, 0.5, 3)
+    with pytest.raises(TokenIndexError, match='embedding gradient: token 777'):
+        check_status()
+    assert torch.equal(dw, want)
+
+
+def test_embedding_sorted_beside_the_lookup_in_a_graph():
+    from mgwfbp_b200.ops.embedding import embedding, embedding_grad
+    n, vocab, dim = 20000, 3001, 510
+    w = torch.randn(vocab, dim, device='cuda', requires_grad=True)
+    t = torch.randint(0, vocab, (n,), device='cuda')
+    dy = torch.randn(n, dim, device='cuda')
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(embedding(t, w), w, dy)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = embedding(t, w)
+        (dw,) = torch.autograd.grad(out, w, dy)
+    for seed in range(5):
+        t.copy_(torch.randint(0, vocab, (n,), device='cuda', generator=torch.Generator(device='cuda').manual_seed(seed)))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, w.detach()[t]) and torch.equal(dw, embedding_grad(dy, t, vocab))

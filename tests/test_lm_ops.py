@@ -208,16 +208,22 @@ def test_native_embedding_refuses_bad_arguments():
     lib = _lib.load(allow_build=False)
     buf = (C.c_int * 64)()
     p = C.addressof(buf)
-    ok = dict(tokens=p, wide=0, n=4, weight=p, ld=4, vocab=8, dim=4, dtype=0, scale=1.0, out=p, status=p, stream=None)
+    ok = dict(tokens=p, wide=0, n=4, weight=p, ld=4, vocab=8, dim=4, dtype=0, scale=1.0, out=p, order=None,
+              padding=-1, status=p, stream=None)
     for bad in (dict(tokens=None), dict(weight=None), dict(out=None), dict(status=None), dict(n=-1), dict(n=1 << 31), dict(vocab=0),
-                dict(vocab=(1 << 31) - 1), dict(dim=0), dict(dtype=3), dict(dtype=-1), dict(ld=3)):
+                dict(vocab=(1 << 31) - 1), dict(dim=0), dict(dtype=3), dict(dtype=-1), dict(ld=3), dict(order=p & ~15),
+                dict(order=p & ~15, n=65537, dim=1024, ld=1024), dict(order=(p & ~15) + 8, n=2000, dim=8192, ld=8192)):
         assert lib.mgw_embedding_fwd(*{**ok, **bad}.values()) == 2, bad
+    for n, there in ((0, False), (1024, False), (1025, True), (65536, True), (65537, False)):
+        assert (lib.mgw_embedding_order_bytes(n, 8, 8192, 0) > 0) == there
+    assert lib.mgw_embedding_order_bytes(2000, 8, 4195, 0) > 0 == lib.mgw_embedding_order_bytes(2000, 8, 4195, 2)   # 32 MB and 16
     need = lib.mgw_embedding_grad_bytes(2000, 8, 4, 0)             # short lists need no scratch memory
     assert need > 0 and lib.mgw_embedding_grad_bytes(0, 8, 4, 0) == 0 and lib.mgw_embedding_grad_bytes(1024, 8, 4, 0) == 0
-    ok = dict(dy=p, ld=4, tokens=p, wide=0, n=2000, vocab=8, dim=4, dtype=0, scale=1.0, padding=-1, dw=p, work=p & ~15, bytes=need,
-              status=p, stream=None)
+    ok = dict(dy=p, ld=4, tokens=p, wide=0, n=2000, vocab=8, dim=4, dtype=0, scale=1.0, padding=-1, order=None, dw=p,
+              work=p & ~15, bytes=need, status=p, stream=None)
     for bad in (dict(dy=None), dict(tokens=None), dict(dw=None), dict(work=None), dict(status=None), dict(bytes=need - 1), dict(ld=3),
-                dict(work=(p & ~15) + 8), dict(dtype=7), dict(dim=-1)):
+                dict(work=(p & ~15) + 8), dict(dtype=7), dict(dim=-1), dict(order=p & ~15),
+                dict(order=(p & ~15) + 8, dim=8192, ld=8192)):
         assert lib.mgw_embedding_grad(*{**ok, **bad}.values()) == 2, bad
 
 
