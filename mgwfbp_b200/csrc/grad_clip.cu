@@ -290,7 +290,7 @@ int launch_norm(const Call& c, int norm) {
     return norm == kNorm2 ? launch<CAP, kNorm2>(c) : norm == kNorm1 ? launch<CAP, kNorm1>(c) : launch<CAP, kNormMax>(c);
 }
 
-constexpr int kSmall = 64, kLarge = 1024;                   // tensors per launch: kernel arguments of 1.4 KB and 21 KB
+constexpr int kSmall = 64, kMedium = 256, kLarge = 1024;    // tensors per launch: kernel arguments of 1.4, 5.4 and 21 KB
 
 int fail(const char* text) {
     mgw_set_last_error(cudaErrorInvalidValue, text, __FILE__, __LINE__);
@@ -321,7 +321,9 @@ extern "C" int mgw_grad_clip(const unsigned long long* ptrs, const long long* nu
         }
         std::vector<int> order(t.size());
         for (size_t i = 0; i < order.size(); ++i) order[i] = (int)i;
-        std::sort(order.begin(), order.end(), [&](int a, int b) { return t[a].ptr < t[b].ptr || (t[a].ptr == t[b].ptr && a < b); });
+        // gradients mostly come in the order of their addresses (one merged buffer, one backward pass)
+        const auto before = [&](int a, int b) { return t[a].ptr < t[b].ptr || (t[a].ptr == t[b].ptr && a < b); };
+        if (!std::is_sorted(order.begin(), order.end(), before)) std::sort(order.begin(), order.end(), before);
         std::vector<char> drop(t.size(), 0);
         uintptr_t end = 0;
         for (size_t k = 0; k < order.size(); ++k) {
@@ -343,7 +345,7 @@ extern "C" int mgw_grad_clip(const unsigned long long* ptrs, const long long* nu
             }
         if (chunks > 0x7fffffffLL) return fail("more than 2^31 chunks of 32 KB");
         const Call c = {t.data(), (int)m, static_cast<double*>(work), scale, max_norm, norm_out, clip != 0 && m > 0, (cudaStream_t)stream};
-        return m <= (size_t)kSmall ? launch_norm<kSmall>(c, norm) : launch_norm<kLarge>(c, norm);
+        return m <= (size_t)kSmall ? launch_norm<kSmall>(c, norm) : m <= (size_t)kMedium ? launch_norm<kMedium>(c, norm) : launch_norm<kLarge>(c, norm);
     } catch (const std::bad_alloc&) {
         return fail("out of host memory");
     }

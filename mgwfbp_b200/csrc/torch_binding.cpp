@@ -6,7 +6,7 @@
 // Why it exists: for a model's window of a few hundred tokens the kernels take 10 to 20 us and the host decides.  Host time of
 // forward and backward, nodes and launches in Python against here: embedding 83 and 49 us, log probabilities 109 and 62,
 // cross entropy 92 and 54; without gradients 11 and 7 us for a lookup, 16 and 8 for log probabilities; clipping 161
-// gradients 88 and 31.  About 40 us of a backward pass are the engine's own: a pass through one view costs as much.
+// gradients 88 and 27.  About 40 us of a backward pass are the engine's own: a pass through one view costs as much.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -389,7 +389,7 @@ std::optional<Tensor> clip_grads(const std::vector<Tensor>& list, bool parameter
     if (parameters) {
         own.reserve(list.size());
         for (const Tensor& p : list)
-            if (p.grad().defined()) own.push_back(p.grad());
+            if (const Tensor& g = p.grad(); g.defined()) own.push_back(g);
     }
     const std::vector<Tensor>& grads = parameters ? own : list;
     if (!clip_supported(grads)) return std::nullopt;
