@@ -818,3 +818,72 @@ def test_embedding_sorted_beside_the_lookup_in_a_graph():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, w.detach()[t]) and torch.equal(dw, embedding_grad(dy, t, vocab))
+
+
+def test_two_threads_on_two_streams():
+    """The host side runs without the interpreter's lock: two threads at once, each on its own stream."""
+    import threading
+    from mgwfbp_b200.ops.clip import clip_grad_norm_
+    from mgwfbp_b200.ops.embedding import check_status, embedding
+    from mgwfbp_b200.ops.logprob import cross_entropy, token_log_probs
+
+    def inputs(seed):
+        gen = torch.Generator(device='cuda').manual_seed(seed)
+        w = torch.randn(3001, 512, device='cuda', generator=gen, requires_grad=True)
+        z = torch.randn(300, 5003, device='cuda', generator=gen, requires_grad=True)
+        return (torch.randint(0, 3001, (17000,), device='cuda', generator=gen), w, torch.randn(17000, 512, device='cuda', generator=gen), z,
+                torch.randint(0, 5003, (300,), device='cuda', generator=gen))
+
+    def once(t, w, dy, z, chosen):
+        out = embedding(t, w, 2.0)
+        (dw,) = torch.autograd.grad(out, w, dy)
+        r = token_log_probs(z, chosen, top=7)
+        (dz,) = torch.autograd.grad(r.logprob.sum() + r.entropy.sum(), z)
+        loss = cross_entropy(z, chosen)
+        (dl,) = torch.autograd.grad(loss, z)
+        p = torch.nn.Parameter(torch.zeros_like(dw))
+        p.grad = dw.clone()
+        norm = clip_grad_norm_([p], 1.0)
+        return [out.detach(), dw, r.logprob.detach(), r.entropy.detach(), r.top_logprob, r.top_tokens, dz, loss.detach(), dl, norm, p.grad]
+    data = [inputs(k) for k in range(2)]
+    want = [once(*d) for d in data]
+    torch.cuda.synchronize()
+    faults = []
+
+    def work(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(15):
+                    got = once(*data[k])
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                        faults.append('thread %d: other values' % k)
+        except Exception as e:                                 # a thread's exception would be lost
+            faults.append('thread %d: %r' % (k, e))
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(120)
+        assert not th.is_alive()
+    assert not faults, faults
+    check_status()
+
+
+def test_native_refusals_carry_their_text():
+    """What the library refuses comes back as the package's error; nothing was launched."""
+    from mgwfbp_b200.ops import counters
+    from mgwfbp_b200.ops._lib import NativeLibraryError
+    from mgwfbp_b200.ops._tokens import native
+    t, w = torch.tensor([0, 1], device='cuda'), torch.zeros(3, 4, device='cuda')
+    before = counters.snapshot()
+    with pytest.raises(NativeLibraryError, match='embedding_grad failed with code 2'):
+        native().embedding_grad(w[:2], t, 0, 1.0, -1)
+    with pytest.raises(NativeLibraryError, match='logprob_fwd failed with code 2'):
+        native().token_log_probs(w[:2], t, -100, 5)            # more than the vocabulary has
+    with pytest.raises(RuntimeError, match='on one device'):
+        native().embedding(t.cpu(), w, 1.0, -1)
+    with pytest.raises(ValueError, match='share memory'):
+        native().clip_grads([w[:2].view(-1), w[1:].view(-1)], False, 0, 1.0, 1.0, True)
+    assert counters.diff(before) == {}
