@@ -12,7 +12,7 @@ import importlib.util
 import os
 from typing import Optional
 
-from .build import BINDING_PATH, CHECKED_LIB_PATH, LIB_PATH, build  # noqa: F401  (re-exported)
+from .build import BINDING_PATH, CHECKED_LIB_PATH, LIB_PATH, build, build_binding  # noqa: F401  (re-exported)
 
 MAX_RANKS = 16
 MAX_CTAS = 296
@@ -131,13 +131,21 @@ def load(allow_build: Optional[bool] = None) -> C.CDLL:
 _binding = None
 
 
-def load_binding():
-    """The module of ``csrc/torch_binding.cpp`` with the loaded library's functions bound to it."""
+def load_binding(allow_build: Optional[bool] = None):
+    """The module of ``csrc/torch_binding.cpp``, built first when that is allowed and needed (:func:`._tokens.native` binds the
+    loaded library's functions to it)."""
     global _binding
     if _binding is None:
         import torch
         if not os.path.isfile(BINDING_PATH):
-            raise NativeLibraryError('%s is missing; run `python -m mgwfbp_b200.ops.build`' % BINDING_PATH)
+            if allow_build is None:
+                allow_build = os.environ.get('MGWFBP_BUILD_ON_IMPORT', '1') != '0'
+            if not allow_build:
+                raise NativeLibraryError('%s is missing; run `python -m mgwfbp_b200.ops.build`' % BINDING_PATH)
+            try:
+                build_binding()
+            except Exception as e:
+                raise NativeLibraryError('could not build %s: %s' % (BINDING_PATH, e)) from e
         spec = importlib.util.spec_from_file_location('_torch_binding', BINDING_PATH)
         try:
             module = importlib.util.module_from_spec(spec)

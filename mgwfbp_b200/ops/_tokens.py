@@ -26,7 +26,7 @@ def native():
     """The module that allocates, launches and records gradients for CUDA tensors (``csrc/torch_binding.cpp``)."""
     global _native
     if _native is None:
-        lib, module = _lib.load(allow_build=False), _lib.load_binding()
+        lib, module = _lib.load(allow_build=False), _lib.load_binding(allow_build=False)
         module.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in _FUNCTIONS}, status_words(), _lib.NativeLibraryError)
         counters.attach(module.launch_counts)
         _native = module

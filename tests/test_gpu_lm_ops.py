@@ -887,3 +887,91 @@ def test_native_refusals_carry_their_text():
     with pytest.raises(ValueError, match='share memory'):
         native().clip_grads([w[:2].view(-1), w[1:].view(-1)], False, 0, 1.0, 1.0, True)
     assert counters.diff(before) == {}
+
+
+@pytest.mark.parametrize('n', [700, 20000, 70000])
+@pytest.mark.parametrize('before', ['copy', 'fill', 'join', 'nothing'])
+def test_captured_behind_other_nodes(n, before):
+    """In a captured graph the launches may follow a copy, a fill, two branches or nothing, not only a kernel."""
+    from mgwfbp_b200.ops.embedding import embedding, embedding_grad
+    vocab, dim = 3001, 500
+    w = torch.randn(vocab, dim, device='cuda', requires_grad=True)
+    t, dy = torch.zeros(n, dtype=torch.int64, device='cuda'), torch.randn(n, dim, device='cuda')
+    source, other = torch.randint(0, vocab, (n,), device='cuda'), torch.zeros(4, device='cuda')
+    side = torch.cuda.Stream()
+
+    def call():
+        main = torch.cuda.current_stream()
+        if before == 'copy':
+            t.copy_(source)
+        elif before == 'fill':
+            other.zero_()
+        elif before == 'join':
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                other.add_(1)
+            t.copy_(source)
+            main.wait_stream(side)
+        a = embedding_grad(dy, t, vocab)
+        out = embedding(t, w)
+        (b,) = torch.autograd.grad(out, w, dy)
+        return a, out, b
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = call()
+    for _ in range(3):
+        source.copy_(torch.randint(0, vocab, (n,), device='cuda'))
+        if before in ('fill', 'nothing'):
+            t.copy_(source)
+        g.replay()
+        torch.cuda.synchronize()
+        want = embedding_grad(dy, source, vocab)
+        assert torch.equal(got[0], want) and torch.equal(got[2], want) and torch.equal(got[1], w.detach()[source])
+
+
+@pytest.mark.parametrize('how', ['offload', 'checkpoint', 'anomaly', 'hooks'])
+def test_graph_features(how):
+    """Saved tensors that are moved away or computed again, anomaly mode and hooks on tensors: the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    from mgwfbp_b200.ops.embedding import embedding
+    from mgwfbp_b200.ops.logprob import cross_entropy, token_log_probs
+    w = torch.randn(777, 96, device='cuda', requires_grad=True)
+    head = torch.randn(1003, 96, device='cuda', requires_grad=True)
+    t, chosen = torch.randint(0, 777, (2000,), device='cuda'), torch.randint(0, 1003, (2000,), device='cuda')
+
+    def model(table, out):
+        z = embedding(t, table, 0.1) @ out.t()
+        r = token_log_probs(z, chosen, top=2)
+        return cross_entropy(z, chosen) + 0.01 * r.entropy.mean() - r.logprob.mean()
+    want = torch.autograd.grad(model(w, head), (w, head))
+    if how == 'offload':
+        with torch.autograd.graph.save_on_cpu():
+            loss = model(w, head)
+        got = torch.autograd.grad(loss, (w, head))
+    elif how == 'checkpoint':
+        got = torch.autograd.grad(checkpoint(model, w, head, use_reentrant=False), (w, head))
+    elif how == 'anomaly':
+        with torch.autograd.set_detect_anomaly(True):
+            got = torch.autograd.grad(model(w, head), (w, head))
+    else:
+        seen = []
+        rows = embedding(t, w, 0.1)
+        rows.register_hook(lambda g: seen.append(g.shape))
+        z = rows @ head.t()
+        z.retain_grad()
+        r = token_log_probs(z, chosen, top=2)
+        loss = cross_entropy(z, chosen)
+        loss.register_hook(lambda g: g * 1.0)
+        got = torch.autograd.grad(loss + 0.01 * r.entropy.mean() - r.logprob.mean(), (w, head))
+        assert seen == [rows.shape]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.inference_mode():
+        assert torch.equal(model(w, head), model(w.detach(), head.detach())) and not model(w, head).requires_grad
+    with torch.no_grad():
+        assert not embedding(t, w).requires_grad and embedding(t, w).grad_fn is None

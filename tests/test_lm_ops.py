@@ -263,3 +263,39 @@ def test_native_clip_refuses_bad_arguments():
     assert b'share memory' in lib.mgw_last_error()
     assert call(ptrs=(4096, 4096), numels=(4, 2)) == 2                 # one inside the other
     assert call(ptrs=(4096, 4096), dtypes=(0, 1)) == 2                 # the same place as two types
+
+
+def test_native_binding_refuses_what_is_not_on_a_gpu():
+    """The functions that allocate and launch take CUDA tensors of the kernels' types only, whoever calls them."""
+    m = _lib.load_binding()
+    t, w = torch.tensor([0, 1]), torch.randn(3, 4)
+    for call in (lambda: m.embedding(t, w, 1.0, -1), lambda: m.embedding_grad(w[:2], t, 3, 1.0, -1),
+                 lambda: m.token_log_probs(w[:2], t, -100, 1), lambda: m.cross_entropy(w[:2], t, -100, True, 1.0)):
+        with pytest.raises(RuntimeError):
+            call()
+    assert not m.clip_supported([w]) and not m.clip_supported([])
+    assert m.clip_grads([w], False, 0, 1.0, 1.0, True) is None
+    assert m.launch_counts() == {}
+    with pytest.raises(TypeError):
+        m.clip_grads([None], False, 0, 1.0, 1.0, True)
+
+
+def test_counters_include_attached_sources():
+    from mgwfbp_b200.ops import counters
+    theirs = {'somewhere': 3}
+    counters.attach(lambda: theirs)
+    try:
+        before = counters.snapshot()
+        theirs['somewhere'] = 5
+        counters.bump('here')
+        assert counters.diff(before) == {'somewhere': 2, 'here': 1}
+        kept = dict(counters._counts)
+        counters.reset()
+        assert counters.total() == 0 and counters.snapshot() == {}
+        theirs['somewhere'] = 6
+        assert counters.total() == 1
+        counters._counts.clear()
+        counters._counts.update(kept)
+    finally:
+        counters._sources.pop()
+        counters._counts.pop('here', None)
