@@ -904,14 +904,15 @@ constexpr long long kResident = 148 * 8;                               // blocks
 constexpr long long kInL2 = 40LL << 20;                               // bytes of rows that are still in L2 when they are read again:
                                                                       // 8192 x 131,072 bf16 782 us, 902 with a block per row
 
-// Blocks per row: one as long as the rows alone give four blocks to every SM, else up to 8 (a portable cluster) that have
-// at least 128 vectors each.  Where rows are read twice (`twice`, the loss and its gradient), as many that the rows in
-// flight stay in L2.
+// Blocks per row: one as soon as the rows alone give 2.7 blocks to every SM, else up to 8 (a portable cluster) that have
+// at least 128 vectors each.  550 rows of 50,000 bf16 with 5 likeliest tokens: 19 us with one, 21 with two; 100 such rows
+// 10.5 with four, 12.5 with eight; 400 rows without them 13 with one or two, and their gradient 15.5 and 14.  Where rows
+// are read twice (`twice`, the loss and its gradient), as many that the rows in flight stay in L2.
 int splits_of(long long rows, int vocab, int dtype, bool twice) {
     const int per = dtype == MGW_F32 ? 4 : 8;
     int splits = 1;
     while (splits < 8 && vocab / per / (splits * 2) >= 128 &&
-           (rows * splits < kResident / 2 || (twice && (rows < kResident / splits ? rows : kResident / splits) * vocab * (16 / per) > kInL2)))
+           (rows * splits < kResident / 3 || (twice && (rows < kResident / splits ? rows : kResident / splits) * vocab * (16 / per) > kInL2)))
         splits *= 2;
     return splits;
 }
