@@ -1,12 +1,12 @@
 // Host side of the language-model operators for CUDA tensors: outputs and workspaces, one launch call, and the nodes of the
 // autograd graph.  The kernels stay in libmgwfbp_b200.so (lm_api.h); their addresses are handed over by bind(), so that this
-// module works with whichever build of that library the process has loaded.  Argument checks that name what is wrong
-// are made by the Python functions in front of this module.
+// module works with whichever build of that library the process has loaded.  Arguments that the kernels do not take give no
+// result here; the Python functions in front of this module then say what is wrong with them.
 //
 // Why it exists: for a model's window of a few hundred tokens the kernels take 10 to 20 us and the host decides.  Host time of
-// forward and backward, nodes and launches in Python against here: embedding 83 and 49 us, log probabilities 109 and 62,
-// cross entropy 92 and 54; without gradients 11 and 7 us for a lookup, 16 and 8 for log probabilities; clipping 161
-// gradients 88 and 27.  About 40 us of a backward pass are the engine's own: a pass through one view costs as much.
+// forward and backward, nodes and launches in Python against here: embedding 83 and 47 us, log probabilities 109 and 57,
+// cross entropy 92 and 51; without gradients 11 and 5 us for a lookup, 16 and 6 for log probabilities; clipping 161
+// gradients 88 and 26.  About 40 us of a backward pass are the engine's own: a pass through one view costs as much.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <optional>
@@ -79,11 +80,14 @@ int type_code(const Tensor& t) {
 
 bool wide(const Tensor& tokens) { return tokens.scalar_type() == at::kLong; }
 
-void need(const Tensor& values, const Tensor& tokens) {
+bool fits(const Tensor& values, const Tensor& tokens) {
     TORCH_CHECK(lib.status != nullptr, "the kernels' library is not bound");
-    TORCH_CHECK(values.is_cuda() && tokens.device() == values.device() && type_code(values) >= 0 && values.dim() >= 1 &&
-                    values.size(-1) >= 1 && (tokens.scalar_type() == at::kInt || wide(tokens)),
-                "CUDA tensors of the kernels' types on one device are needed");
+    return values.is_cuda() && tokens.device() == values.device() && type_code(values) >= 0 && values.dim() >= 1 && values.size(-1) >= 1 &&
+           values.size(-1) <= 1LL << 30 && (tokens.scalar_type() == at::kInt || wide(tokens)) && tokens.numel() <= 0x7fffffffLL;
+}
+// one row of values for each token
+bool fits_rows(const Tensor& values, const Tensor& tokens) {
+    return fits(values, tokens) && values.dim() == tokens.dim() + 1 && values.sizes().slice(0, tokens.dim()) == tokens.sizes();
 }
 
 // The tensor's device is the current one while this lives; launches go to its current stream.
@@ -134,7 +138,6 @@ Tensor once_differentiable(Tensor g, bool wanted) {
 // ------------------------------------------------------------------------------------------------------- embedding
 // order: where it is given and the sizes are such, it becomes the sorted list for the gradient.
 Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding, Tensor* order) {
-    need(weight, tokens);
     at::NoGradGuard no_grad;
     Place on(weight);
     const Rows w(weight);
@@ -153,7 +156,6 @@ Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, double scal
 }
 
 Tensor embedding_gradient(const Tensor& dy, const Tensor& tokens, int64_t vocab, double scale, int64_t padding, const Tensor& order) {
-    need(dy, tokens);
     at::NoGradGuard no_grad;
     Place on(dy);
     const Rows g(dy);
@@ -169,7 +171,8 @@ Tensor embedding_gradient(const Tensor& dy, const Tensor& tokens, int64_t vocab,
     return dw;
 }
 
-Tensor embedding_grad(const Tensor& dy, const Tensor& tokens, int64_t vocab, double scale, int64_t padding) {
+std::optional<Tensor> embedding_grad(const Tensor& dy, const Tensor& tokens, int64_t vocab, double scale, int64_t padding) {
+    if (!fits_rows(dy, tokens) || vocab < 1 || vocab > 0x7ffffffeLL) return std::nullopt;
     return embedding_gradient(dy, tokens, vocab, scale, padding, Tensor());
 }
 
@@ -193,7 +196,8 @@ struct EmbeddingBackward : Node {
     std::string name() const override { return "EmbeddingBackward"; }
 };
 
-Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+std::optional<Tensor> embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+    if (!fits(weight, tokens) || weight.dim() != 2 || weight.size(0) < 1 || weight.size(0) > 0x7ffffffeLL) return std::nullopt;
     const bool train = differentiable(weight);
     Tensor order, out = embedding_forward(tokens, weight, scale, padding, train ? &order : nullptr);
     if (train) {
@@ -255,9 +259,10 @@ struct TokenLogProbsBackward : Node {
     std::string name() const override { return "TokenLogProbsBackward"; }
 };
 
-std::tuple<Tensor, Tensor, std::optional<Tensor>, std::optional<Tensor>> token_log_probs(const Tensor& logits, const Tensor& tokens,
-                                                                                         int64_t ignore, int64_t top) {
-    need(logits, tokens);
+typedef std::tuple<Tensor, Tensor, std::optional<Tensor>, std::optional<Tensor>> LogProbs;
+
+std::optional<LogProbs> token_log_probs(const Tensor& logits, const Tensor& tokens, int64_t ignore, int64_t top) {
+    if (!fits_rows(logits, tokens) || top < 0 || top > std::min<int64_t>(32, logits.size(-1))) return std::nullopt;
     const bool train = differentiable(logits);
     Tensor logprob, h, stats;
     std::optional<Tensor> best, which;
@@ -291,7 +296,7 @@ std::tuple<Tensor, Tensor, std::optional<Tensor>, std::optional<Tensor>> token_l
         node->ignore = ignore;
         torch::autograd::set_history({logprob, h}, node);
     }
-    return {logprob, h, best, which};
+    return LogProbs(logprob, h, best, which);
 }
 
 // --------------------------------------------------------------------------------------------------- cross entropy
@@ -337,8 +342,8 @@ struct CrossEntropyBackward : Node {
     std::string name() const override { return "CrossEntropyBackward"; }
 };
 
-Tensor cross_entropy(const Tensor& logits, const Tensor& tokens, int64_t ignore, bool mean, double expected) {
-    need(logits, tokens);
+std::optional<Tensor> cross_entropy(const Tensor& logits, const Tensor& tokens, int64_t ignore, bool mean, double expected) {
+    if (!fits_rows(logits, tokens)) return std::nullopt;
     const bool train = differentiable(logits);
     Tensor loss, work, dz;
     {

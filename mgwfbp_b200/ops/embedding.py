@@ -91,11 +91,13 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     """``scale * weight[tokens]``, shape ``tokens.shape + [width]``, in ``weight``'s type (products in fp32, rounded once;
     ``scale == 1`` copies the rows).  ``tokens``: int32 or int64 of any shape; ``weight``: ``[vocabulary, width]``, rows may
     lie further apart than their width.  ``padding_idx`` only matters to the gradient: that row gets none."""
-    _check(tokens, weight)
-    padding, scale = _padding(padding_idx, weight.shape[0]), float(scale)
+    padding = -1 if padding_idx is None or weight.dim() != 2 else _padding(padding_idx, weight.shape[0])
     if weight.is_cuda:
-        return native().embedding(tokens, weight, scale, padding)
-    return _EmbeddingCPU.apply(tokens, weight, scale, padding)
+        out = native().embedding(tokens, weight, scale, padding)
+        if out is not None:                                    # else the check below says why
+            return out
+    _check(tokens, weight)
+    return _EmbeddingCPU.apply(tokens, weight, float(scale), padding)
 
 
 class FusedEmbedding(nn.Embedding):

@@ -80,10 +80,12 @@ def _reference(logits: torch.Tensor, tokens: torch.Tensor, ignore: int, top: int
 def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ignore_index: int = -100) -> TokenLogProbs:
     """Log probability of ``tokens`` (int32 or int64, any shape) under ``softmax(logits)``, entropy of every row, and its
     ``top`` (0 to 32) likeliest tokens.  See the module for masks, padding and what is refused."""
+    if logits.is_cuda:
+        found = native().token_log_probs(logits, tokens, int(ignore_index), top)
+        if found is not None:                                  # else the check below says why
+            return TokenLogProbs(*found)
     _check(logits, tokens, top)
-    if not logits.is_cuda:
-        return TokenLogProbs(*_reference(logits, tokens, int(ignore_index), top))
-    return TokenLogProbs(*native().token_log_probs(logits, tokens, int(ignore_index), top))
+    return TokenLogProbs(*_reference(logits, tokens, int(ignore_index), top))
 
 
 def cross_entropy(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int = -100, reduction: str = 'mean',
@@ -96,17 +98,19 @@ def cross_entropy(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int 
     at the cost of another pass over the logits."""
     if reduction not in ('mean', 'sum', 'none'):
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
-    _check(logits, tokens)
     if reduction == 'none':
         return -token_log_probs(logits, tokens, 0, ignore_index).logprob
-    if not logits.is_cuda:
-        logprob = _reference(logits, tokens, int(ignore_index), 0)[0]
-        total = -logprob.sum()
-        return total / (tokens != ignore_index).sum() if reduction == 'mean' else total
     expected = float(expected_grad)
     if not math.isfinite(expected):
         raise ValueError('expected_grad must be finite, got %r' % (expected_grad,))
-    return native().cross_entropy(logits, tokens, int(ignore_index), reduction == 'mean', expected)
+    if logits.is_cuda:
+        loss = native().cross_entropy(logits, tokens, int(ignore_index), reduction == 'mean', expected)
+        if loss is not None:                                   # else the check below says why
+            return loss
+    _check(logits, tokens)
+    logprob = _reference(logits, tokens, int(ignore_index), 0)[0]
+    total = -logprob.sum()
+    return total / (tokens != ignore_index).sum() if reduction == 'mean' else total
 
 
 class FusedCrossEntropyLoss(nn.CrossEntropyLoss):

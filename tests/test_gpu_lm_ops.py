@@ -871,21 +871,51 @@ def test_two_threads_on_two_streams():
     check_status()
 
 
-def test_native_refusals_carry_their_text():
-    """What the library refuses comes back as the package's error; nothing was launched."""
-    from mgwfbp_b200.ops import counters
-    from mgwfbp_b200.ops._lib import NativeLibraryError
-    from mgwfbp_b200.ops._tokens import native
-    t, w = torch.tensor([0, 1], device='cuda'), torch.zeros(3, 4, device='cuda')
+def test_native_errors_carry_their_text():
+    """What the library refuses comes back as the package's error, from the caller's thread and from the backward pass."""
+    import ctypes as C
+    from mgwfbp_b200.ops import _lib, _tokens, counters
+    m, lib = _tokens.native(), _lib.load(allow_build=False)
+    t, w = torch.tensor([0, 1], device='cuda'), torch.zeros(3, 4, device='cuda', requires_grad=True)
+    z = torch.zeros(2, 4, device='cuda', requires_grad=True)
+    out, loss = m.embedding(t, w, 1.0, -1), m.cross_entropy(z, t, -100, True, 1.0)
     before = counters.snapshot()
-    with pytest.raises(NativeLibraryError, match='embedding_grad failed with code 2'):
-        native().embedding_grad(w[:2], t, 0, 1.0, -1)
-    with pytest.raises(NativeLibraryError, match='logprob_fwd failed with code 2'):
-        native().token_log_probs(w[:2], t, -100, 5)            # more than the vocabulary has
-    with pytest.raises(RuntimeError, match='on one device'):
-        native().embedding(t.cpu(), w, 1.0, -1)
     with pytest.raises(ValueError, match='share memory'):
-        native().clip_grads([w[:2].view(-1), w[1:].view(-1)], False, 0, 1.0, 1.0, True)
+        m.clip_grads([w.detach()[:2].view(-1), w.detach()[1:].view(-1)], False, 0, 1.0, 1.0, True)
+    real = {name: C.cast(getattr(lib, name), C.c_void_p).value for name in _tokens._FUNCTIONS}
+    failing = C.CFUNCTYPE(C.c_int)(lambda: 7)                  # stands in for every launch: nothing reaches the GPU
+    fake = {k: v if k == 'mgw_last_error' or k.endswith('_bytes') else C.cast(failing, C.c_void_p).value for k, v in real.items()}
+    m.bind(fake, _tokens.status_words(), _lib.NativeLibraryError)
+    try:
+        for what, call in (('embedding_fwd', lambda: m.embedding(t, w, 1.0, -1)), ('embedding_grad', lambda: m.embedding_grad(z, t, 3, 1.0, -1)),
+                           ('logprob_fwd', lambda: m.token_log_probs(z, t, -100, 1)),
+                           ('cross_entropy_fwd', lambda: m.cross_entropy(z, t, -100, True, 1.0)),
+                           ('grad_clip', lambda: m.clip_grads([z.detach()], False, 0, 1.0, 1.0, True))):
+            with pytest.raises(_lib.NativeLibraryError, match='%s failed with code 7' % what):
+                call()
+        for what, x in (('embedding_grad', out.sum()), ('cross_entropy_bwd', loss)):
+            with pytest.raises(RuntimeError, match='%s failed with code 7' % what):
+                x.backward()
+    finally:
+        m.bind(real, _tokens.status_words(), _lib.NativeLibraryError)
+    assert counters.diff(before) == {}
+    assert torch.equal(m.embedding(t, w, 1.0, -1), w[t])
+
+
+def test_native_calls_leave_other_arguments_alone():
+    """No result, and no launch, for what the kernels do not take: the functions in front say why."""
+    from mgwfbp_b200.ops import counters
+    from mgwfbp_b200.ops._tokens import native
+    m, t, w = native(), torch.tensor([0, 1], device='cuda'), torch.zeros(3, 4, device='cuda')
+    before = counters.snapshot()
+    for got in (m.embedding(t.cpu(), w, 1.0, -1), m.embedding(t, w.double(), 1.0, -1), m.embedding(t, w[0], 1.0, -1),
+                m.embedding(t.float(), w, 1.0, -1), m.embedding(t, w[:0], 1.0, -1), m.embedding(t, w[:, :0], 1.0, -1),
+                m.embedding_grad(w[:2], t, 0, 1.0, -1), m.embedding_grad(w, t, 3, 1.0, -1), m.token_log_probs(w, t, -100, 1),
+                m.token_log_probs(w[:2], t, -100, 5), m.token_log_probs(w[:2], t, -100, -1), m.token_log_probs(w[:2], t[:, None], -100, 1),
+                m.cross_entropy(w, t, -100, True, 1.0), m.cross_entropy(w[:2].double(), t, -100, True, 1.0),
+                m.clip_grads([w.double()], False, 0, 1.0, 1.0, True), m.clip_grads([w[:, ::2]], False, 0, 1.0, 1.0, True),
+                m.clip_grads([w, w.cpu()], False, 0, 1.0, 1.0, True), m.clip_grads([], False, 0, 1.0, 1.0, True)):
+        assert got is None
     assert counters.diff(before) == {}
 
 
