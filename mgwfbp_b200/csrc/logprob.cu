@@ -15,8 +15,8 @@
 //
 // Measured (device time): 4099 rows of 50,261 bf16 logits with 20 alternatives 84 us (413 MB; 67 us without the
 // alternatives, 63 us is the floor), 700 x 10,000 fp32 with 5 of them 9.6 us (7.3 without), 2048 x 32,000 bf16 26 us and its
-// gradient 45 us (5.8 TB/s).  Mean loss with gradient of 8192 x 131,072 bf16 780 us (4.3 GB, 5.5 TB/s: logits once from
-// memory, once from L2, gradient once to memory), 700 x 10,000 fp32 21 us.  Before the pairs, with 256 threads per block
+// gradient 45 us (5.8 TB/s).  Mean loss with gradient of 8192 x 131,072 bf16 775 us (4.3 GB, 5.5 TB/s: logits once from
+// memory, once from L2, gradient once to memory), 700 x 10,000 fp32 20 us.  Before the pairs, with 256 threads per block
 // and plain loads, these were 184, 15, 38 + 61 and 1017 us.
 //
 // The likeliest tokens come out of the same pass.  Every thread knows the largest of its logits, so the K-th largest of the
@@ -34,6 +34,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxTop = 32;
+constexpr int kMaxSplits = 8;              // blocks of a cluster that share a row
 constexpr int kThreads = 128;              // 8 blocks per SM; with 64 threads the first case above takes 105 us, not 99
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;                 // 16-byte vectors of a thread in a batch
@@ -712,8 +713,14 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
             cg::cluster_group cluster = cg::this_cluster();
             if (threadIdx.x == 0) of_block = x;
             cluster.sync();
-            x = *cluster.map_shared_rank(&of_block, 0);
-            for (int k = 1; k < a.splits; ++k) x = join<ENT>(x, *cluster.map_shared_rank(&of_block, k));
+            Stats each[kMaxSplits];                                  // all on their way before the first is needed
+#pragma unroll
+            for (int k = 0; k < kMaxSplits; ++k)
+                if (k < a.splits) each[k] = *cluster.map_shared_rank(&of_block, k);
+            x = each[0];
+#pragma unroll
+            for (int k = 1; k < kMaxSplits; ++k)
+                if (k < a.splits) x = join<ENT>(x, each[k]);
         }
         if (careful<T>(x.m)) x = careful_row(row.z, a.vocab, parts);
         const bool fine = fabsf(x.m) < INFINITY;
@@ -731,8 +738,14 @@ __global__ void __launch_bounds__(kThreads, 8) logprob_fwd_kernel(RowArgs a) {
                 cg::cluster_group cluster = cg::this_cluster();
                 if (warp == 0) block_list[lane] = mine;
                 cluster.sync();
-                if (part == 0 && warp == 0)
-                    for (int k = 1; k < a.splits; ++k) mine = merge_lists(mine, *cluster.map_shared_rank(&block_list[lane], k));
+                if (part == 0 && warp == 0) {                        // likewise
+                    Key other[kMaxSplits - 1];
+#pragma unroll
+                    for (int k = 1; k < kMaxSplits; ++k) other[k - 1] = k < a.splits ? *cluster.map_shared_rank(&block_list[lane], k) : (Key)0;
+#pragma unroll
+                    for (int k = 1; k < kMaxSplits; ++k)
+                        if (k < a.splits) mine = merge_lists(mine, other[k - 1]);
+                }
             }
             if (part == 0 && warp == 0 && lane < a.top && mine != 0) {      // key 0 is no entry: never an index
                 const int j = (int)(0xffffffffu - (uint32_t)mine);
@@ -911,7 +924,7 @@ constexpr long long kInL2 = 40LL << 20;                               // bytes o
 int splits_of(long long rows, int vocab, int dtype, bool twice) {
     const int per = dtype == MGW_F32 ? 4 : 8;
     int splits = 1;
-    while (splits < 8 && vocab / per / (splits * 2) >= 128 &&
+    while (splits < kMaxSplits && vocab / per / (splits * 2) >= 128 &&
            (rows * splits < kResident / 3 || (twice && (rows < kResident / splits ? rows : kResident / splits) * vocab * (16 / per) > kInL2)))
         splits *= 2;
     return splits;
